@@ -401,6 +401,51 @@ def dropout_add_layer_norm(h: torch.Tensor, residual: torch.Tensor, norm: nn.Lay
         return _DropoutAddLayerNormFn.apply(h, residual, norm.weight, norm.bias, float(p), bool(training), float(norm.eps))
 
 
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                   cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
+                   interleaved: bool = False):
+    """RMS norm of every query and key head and the rotation by position, in one pass over both (``(q', k')``).
+
+    ``q`` ``[batch, length, heads, head_dim]`` and ``k`` ``[batch, length, key_heads, head_dim]`` may be slices of one packed
+    projection; ``q_weight`` / ``k_weight`` ``[head_dim]`` are the norms' weights (``None``: ones).  ``cos`` / ``sin``
+    ``[positions, rotated / 2]`` rotate the first ``rotated`` dimensions in pairs ``(i, i + rotated / 2)``, or ``(2i, 2i + 1)`` with
+    ``interleaved``; the other dimensions are normalised only.  ``positions`` (int64 / int32, ``[batch, length]`` or ``[length]``)
+    chooses the rows of the tables, by default ``0 .. length - 1``; a token whose position lies outside them (a padding token
+    marked with -1) gives zeros and gets zero gradients.  The results are contiguous and have the inputs' dtype; sums are taken in
+    fp32.  Differentiable in ``q``, ``k`` and the weights."""
+    return torch.ops.catch_b200.qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+
+
+def relative_bias_softmax(scores: torch.Tensor, table: torch.Tensor, mask: Optional[torch.Tensor] = None, *, scale: float = 1.0,
+                          bidirectional: bool = True, max_distance: int = 128, query_offset: int = 0) -> torch.Tensor:
+    """``softmax(scale * scores + bias + mask)`` over the keys, where the bias is learned for buckets of relative positions.
+
+    ``scores`` ``[batch, heads, queries, keys]``; ``table`` ``[buckets, heads]``.  Key ``j`` lies ``j - (i + query_offset)`` from query
+    ``i`` (one query behind a cache of ``n`` keys: ``query_offset = n - 1``).  With ``bidirectional`` the upper half of the buckets
+    is for keys after the query, else those share bucket 0.  Of a side's ``n`` buckets the distances below ``n // 2`` have one each,
+    farther ones share the rest by logarithm, and all from ``max_distance`` on share the last.  ``mask`` broadcasts to the
+    scores: bool (``True`` keeps a key) or floating (added; ``-inf`` excludes a key whatever its score holds).  A row without any key left
+    gives zeros.  Differentiable in ``scores`` and ``table``; the bias is never stored as a matrix."""
+    return torch.ops.catch_b200.relative_bias_softmax(scores, table, mask, scale, bidirectional, max_distance, query_offset)[0]
+
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def top_logits_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor, *, temperature: float = 1.0,
+                            reduction: str = "mean") -> torch.Tensor:
+    """Distillation loss against a teacher of which the largest logits of every row are kept.
+
+    ``logits`` ``[rows, vocabulary]``; ``teacher_logits`` / ``teacher_index`` ``[rows, kept]`` are the teacher's values and their places in
+    the vocabulary (``torch.topk`` of its logits).  A row's loss is ``temperature ** 2 * sum(p * (log p - log q))`` with ``p`` the softmax
+    of the kept logits and ``q`` the student's softmax over the whole vocabulary, both at ``temperature``.  An entry whose index is
+    negative is absent, and a row without entries counts nothing: not in the loss, the gradient or the mean.  ``reduction``:
+    ``"mean"`` over the rows that count, ``"sum"`` or ``"none"``; the loss is fp32.  Differentiable in ``logits``."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"top_logits_distillation: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    return torch.ops.catch_b200.top_logits_distillation(logits, teacher_logits, teacher_index, temperature, _REDUCTIONS[reduction])
+
+
 def _feeds_only(node: fx.Node, consumer: fx.Node) -> bool:
     return len(node.users) == 1 and next(iter(node.users)) is consumer
 

@@ -523,6 +523,91 @@ B200_API int b200_nms_mask(const float* sorted_boxes, int n, float iou_threshold
 B200_API int b200_depthwise_conv(int pass, const void* x, const void* w, void* y, int dtype, const long long* dims,
                                  const int* conv, const long long* x_strides, const long long* y_strides, void* stream);
 
+// ---- transformer rows: query / key norm + rotation, biased softmax, distillation loss ------------
+// RMS norm of every query and key head and the rotation by position (qk_norm_rotary.cu).  x and dy are [B, L, heads, D] with
+// any strides and a dense last dimension; out is contiguous [B, L, heads, D].  R: rotated dimensions (even, <= D).
+#define B200_QK_MAX_HEAD_DIM 512
+typedef struct B200QkSide {
+  const void* x;
+  const void* dy;            // backward
+  void* out;                 // forward: y; backward: dx
+  const void* weight;        // [D] f32 / bf16 / f16, or null
+  void* dweight;             // backward: [D] in weight_dtype, or null
+  int weight_dtype;
+  int heads;
+  int64_t x_stride[3], dy_stride[3];  // of B, L and heads, in elements
+} B200QkSide;
+typedef struct B200QkNormRotary {
+  B200QkSide side[2];        // queries, keys
+  int64_t B, L;
+  int D, R, dtype, interleaved;
+  const float* cos;          // [table_rows][R / 2]
+  const float* sin;
+  int64_t table_rows;
+  const void* positions;     // [B, L] of int64 / int32 with pos_stride, or null: 0 .. L-1.  Outside the tables: zeros are
+  int positions_dtype;       // written for the token and *bad_flag is set
+  int64_t pos_stride[2];
+  int* bad_flag;             // may be null
+  float eps;
+} B200QkNormRotary;
+B200_API int b200_qk_norm_rotary_fwd(const B200QkNormRotary* p, void* stream);
+B200_API long long b200_qk_norm_rotary_workspace(const B200QkNormRotary* p);  // bytes that the backward needs
+B200_API int b200_qk_norm_rotary_bwd(const B200QkNormRotary* p, void* workspace, void* stream);
+
+// Softmax over scores [B, H, Lq, Lk] with a relative position bias (bias_softmax.cu).
+#define B200_MAX_FAR_BUCKETS 128
+#define B200_MAX_BIAS_DISTANCE 8192
+typedef struct B200RelativeBuckets {
+  int bidirectional;         // keys after the query have buckets of their own (the upper half)
+  int per_side;              // buckets for one side
+  int exact;                 // distances below have a bucket each
+  int max_distance;          // distances from here on share the last bucket
+  int first[B200_MAX_FAR_BUCKETS];  // smallest distance of the far bucket exact + k
+} B200RelativeBuckets;
+typedef struct B200BiasSoftmax {
+  const void* scores;        // scores, grad and out share strides and begin on 16-byte boundaries; last dimension dense
+  const void* grad;          // backward: gradient of the probabilities
+  void* out;                 // forward: probabilities; backward: gradient of the scores
+  float* stats;              // [B, H, Lq, 2]: maximum and 1 / sum; forward: written, or null
+  const void* table;         // [buckets, H] f32 / bf16 / f16, dense
+  void* dtable;              // backward: like table, or null
+  const void* mask;          // bool (true keeps) or additive f32 / bf16 / f16, or null
+  int64_t stride[3];         // of B, H, Lq in elements
+  int64_t mask_stride[4];    // 0 along broadcast dimensions
+  int dtype, table_dtype, mask_dtype;
+  int B, H, Lq, Lk;
+  int query_offset;          // query i is at position i + query_offset of the keys
+  float scale;
+  B200RelativeBuckets buckets;
+} B200BiasSoftmax;
+B200_API int b200_bias_softmax_fwd(const B200BiasSoftmax* p, void* stream);
+B200_API long long b200_bias_softmax_workspace(const B200BiasSoftmax* p);  // bytes that the backward needs
+B200_API int b200_bias_softmax_bwd(const B200BiasSoftmax* p, void* workspace, void* stream);
+
+// Distillation loss against a teacher's top K logits (distill_loss.cu).
+#define B200_DISTILL_MAX_K 1024
+typedef struct B200Distill {
+  const void* logits;        // [N][ld], V columns used; f32 / bf16 / f16
+  const void* teacher;       // [N][teacher_ld], K columns; f32 / bf16 / f16
+  const void* index;         // [N][index_ld], K columns; int64 / int32; negative: absent.  An index >= V is taken as absent
+  int* bad_flag;             // and sets *bad_flag (may be null)
+  int64_t ld, teacher_ld, index_ld;
+  int64_t N, V;
+  int K, dtype, teacher_dtype, index_dtype;
+  float temperature, inv_temperature;
+  float* row_loss;           // [N]
+  float* loss;               // sum (or mean) of the rows' losses, or null
+  float* stats;              // [N, 2]: maximum and sum of exponentials; forward: written, or null
+  float* count;              // for a mean: the number of rows with entries (the forward writes it); else null
+  void* dlogits;             // [N][ld] of dtype, at the same 16-byte phase as logits; forward: written with factor 1, or null
+  const float* grad;         // backward: the factor, one for each row (grad_ld apart) or one for all
+  int64_t grad_ld;
+  int grad_per_row;
+  int skip_factor_one;       // backward: dlogits already holds the gradient for factor 1
+} B200Distill;
+B200_API int b200_distill_fwd(const B200Distill* p, void* stream);
+B200_API int b200_distill_bwd(const B200Distill* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

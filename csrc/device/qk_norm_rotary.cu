@@ -1,0 +1,400 @@
+// RMS norm of every query and key head with the rotation by position in the same pass, forward and backward.
+//
+//   r = 1 / sqrt(mean(x^2) + eps),  n = x r w,  y = turn(n)      for every head x of every token, D = head dimension
+//   turn: the first R dimensions in pairs (a, b) -> (a cos - b sin, b cos + a sin), the others unchanged; the pairs are
+//   (i, i + R/2), or (2i, 2i + 1) when interleaved; cos / sin come from tables, row = the token's position
+//   backward: g = turn by the negative angle of dy;  dw = sum g x r;  dx = r (g w - x r^2 mean(g w x))
+//
+// Bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.  The norm is recomputed from x in
+// the backward, which has to read x anyway, so nothing is kept between the two.
+//
+// A head is split into units of two vectors of VEC elements, chosen so that a rotation never leaves a unit: for split
+// halves the vectors lie R/2 apart, for interleaved pairs they are neighbours.  A unit sits in one lane, so the rotation
+// needs no exchange, and the norm is one reduction over the group of lanes (a power of two) that shares a head: at D = 64
+// in 16 bits a head is four lanes with two 16-byte loads each, eight heads per warp.  A group walks over some heads
+// of one token and keeps the token's cos / sin and the weight in registers.
+#include "kernels_api.h"
+#include "row_vec.cuh"
+
+namespace {
+
+using namespace rowvec;
+
+constexpr int kThreads = 256;
+
+// One side of the pass: the queries or the keys.
+struct Side {
+  const void* x;
+  const void* dy;       // backward
+  void* out;            // y or dx, contiguous [tokens, heads, D]
+  const void* weight;   // [D] or null
+  float* dw_partial;    // backward: [blocks of this side][D], or null
+  long long xs_b, xs_l, xs_h, gs_b, gs_l, gs_h;  // strides of x and dy in elements
+  int heads, weight_dtype;
+  int heads_per_item, items_per_token;
+  unsigned items;       // tokens * items_per_token
+  int blocks;
+};
+struct Args {
+  Side side[2];
+  const float* cos;
+  const float* sin;
+  const void* positions;  // int64 / int32, or null: the token's place in its sequence
+  long long pos_b, pos_l;
+  int pos_is_64;
+  long long table_rows;
+  int* bad_flag;        // set when a position lies outside the tables; may be null
+  unsigned L;
+  int D, R, group;      // lanes per head
+  float eps;
+};
+
+__device__ __forceinline__ float weight_at(const void* w, int dt, int i) {
+  if (dt == B200_F32) return static_cast<const float*>(w)[i];
+  if (dt == B200_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
+  return __half2float(static_cast<const __half*>(w)[i]);
+}
+
+// Where the two vectors of a unit begin, and whether they rotate.
+template <int VEC, bool INTER>
+__device__ __forceinline__ void place(int unit, int R, int& lo, int& hi, bool& rot) {
+  const int first = unit * 2 * VEC;
+  if (INTER || first >= R) { lo = first; hi = first + VEC; rot = first < R; }
+  else { lo = unit * VEC; hi = R / 2 + unit * VEC; rot = true; }
+}
+
+template <int VEC, bool INTER>
+__device__ __forceinline__ void turn(float (&a)[VEC], float (&b)[VEC], const float (&c)[VEC], const float (&s)[VEC]) {
+  if (!INTER) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const float x = a[k], y = b[k];
+      a[k] = x * c[k] - y * s[k];
+      b[k] = y * c[k] + x * s[k];
+    }
+  } else {
+    // the unit is one run of 2 VEC elements: pair i is (2i, 2i + 1)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      float& x = 2 * i < VEC ? a[(2 * i) % VEC] : b[(2 * i) % VEC];
+      float& y = 2 * i + 1 < VEC ? a[(2 * i + 1) % VEC] : b[(2 * i + 1) % VEC];
+      const float u = x, v = y;
+      x = u * c[i] - v * s[i];
+      y = v * c[i] + u * s[i];
+    }
+  }
+}
+
+template <typename T, int VEC, int CH, bool INTER, bool BWD>
+__global__ void __launch_bounds__(kThreads) qk_norm_rotary_kernel(const __grid_constant__ Args p) {
+  extern __shared__ float sh_dw[];  // backward: [warps][D]
+  const bool keys = blockIdx.x >= (unsigned)p.side[0].blocks;
+  const Side& sd = p.side[keys ? 1 : 0];
+  const unsigned block = keys ? blockIdx.x - p.side[0].blocks : blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int G = p.group, gl = threadIdx.x & (G - 1);
+  const unsigned groups_per_block = kThreads / G;
+  const int units = p.D / (2 * VEC);
+  const T* x = static_cast<const T*>(sd.x);
+  const T* dy = static_cast<const T*>(sd.dy);
+  T* out = static_cast<T*>(sd.out);
+  const float inv_d = 1.f / (float)p.D;
+
+  int lo[CH], hi[CH];
+  bool rot[CH], on[CH];
+  float wl[CH][VEC], wh[CH][VEC];
+  float dl[CH][VEC], dh[CH][VEC];  // backward: this lane's part of dw
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int u = gl + c * G;
+    on[c] = u < units;
+    place<VEC, INTER>(on[c] ? u : 0, p.R, lo[c], hi[c], rot[c]);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      wl[c][k] = sd.weight ? weight_at(sd.weight, sd.weight_dtype, lo[c] + k) : 1.f;
+      wh[c][k] = sd.weight ? weight_at(sd.weight, sd.weight_dtype, hi[c] + k) : 1.f;
+      dl[c][k] = dh[c][k] = 0.f;
+    }
+  }
+
+  // All groups of a warp run the same number of rounds, since the reductions take the whole warp.
+  const unsigned stride = (unsigned)sd.blocks * groups_per_block;
+  const unsigned first = block * groups_per_block + threadIdx.x / G;
+  const unsigned warp_first = block * groups_per_block + (threadIdx.x & ~31u) / G;
+  for (unsigned long long base = warp_first, item = first; base < sd.items; base += stride, item += stride) {
+    const bool live = item < sd.items;
+    const unsigned token = live ? (unsigned)item / (unsigned)sd.items_per_token : 0;
+    const unsigned part = live ? (unsigned)item % (unsigned)sd.items_per_token : 0;
+    const unsigned b = token / p.L, l = token % p.L;
+    long long pos = l;
+    if (p.positions) {
+      const long long at = b * p.pos_b + l * p.pos_l;
+      pos = p.pos_is_64 ? static_cast<const long long*>(p.positions)[at] : (long long)static_cast<const int*>(p.positions)[at];
+    }
+    const bool inside = pos >= 0 && pos < p.table_rows;
+    if (live && !inside && p.bad_flag && gl == 0) *p.bad_flag = 1;
+    float cs[CH][VEC], sn[CH][VEC];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) { cs[c][k] = 1.f; sn[c][k] = 0.f; }
+      if (live && inside && on[c] && rot[c]) {
+        const long long at = pos * (p.R / 2) + (INTER ? lo[c] / 2 : lo[c]);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          cs[c][k] = __ldg(p.cos + at + k);
+          sn[c][k] = BWD ? -__ldg(p.sin + at + k) : __ldg(p.sin + at + k);
+        }
+      }
+    }
+    const int h0 = (int)part * sd.heads_per_item;
+    const int hn = live ? min(sd.heads_per_item, sd.heads - h0) : 0;
+    const T* xt = x + b * sd.xs_b + l * sd.xs_l;
+    const T* gt = BWD ? dy + b * sd.gs_b + l * sd.gs_l : nullptr;
+    T* ot = out + (long long)token * sd.heads * p.D;
+    for (int i = 0; i < sd.heads_per_item; ++i) {
+      const bool act = i < hn;
+      const int h = h0 + (act ? i : 0);
+      float a[CH][VEC], z[CH][VEC];
+      float ss = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) a[c][k] = z[c][k] = 0.f;
+        if (act && on[c]) {
+          load<T, VEC>(xt + h * sd.xs_h + lo[c], a[c]);
+          load<T, VEC>(xt + h * sd.xs_h + hi[c], z[c]);
+        }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) ss += a[c][k] * a[c][k] + z[c][k] * z[c][k];
+      }
+      if (!BWD) {
+        const float r = rsqrtf(group_sum(ss, G) * inv_d + p.eps);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            a[c][k] = inside ? a[c][k] * (r * wl[c][k]) : 0.f;
+            z[c][k] = inside ? z[c][k] * (r * wh[c][k]) : 0.f;
+          }
+          turn<VEC, INTER>(a[c], z[c], cs[c], sn[c]);
+          if (act && on[c]) {
+            store<T, VEC>(ot + (long long)h * p.D + lo[c], a[c]);
+            store<T, VEC>(ot + (long long)h * p.D + hi[c], z[c]);
+          }
+        }
+      } else {
+        float ga[CH][VEC], gz[CH][VEC];
+        float dot = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) ga[c][k] = gz[c][k] = 0.f;
+          if (act && on[c] && inside) {
+            load<T, VEC>(gt + h * sd.gs_h + lo[c], ga[c]);
+            load<T, VEC>(gt + h * sd.gs_h + hi[c], gz[c]);
+          }
+          turn<VEC, INTER>(ga[c], gz[c], cs[c], sn[c]);
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) dot += ga[c][k] * wl[c][k] * a[c][k] + gz[c][k] * wh[c][k] * z[c][k];
+        }
+        const float r = rsqrtf(group_sum(ss, G) * inv_d + p.eps);
+        const float m = group_sum(dot, G) * inv_d * r * r;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          float da[VEC], dz[VEC];
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            if (act && inside) {
+              dl[c][k] += ga[c][k] * a[c][k] * r;
+              dh[c][k] += gz[c][k] * z[c][k] * r;
+            }
+            da[k] = inside ? r * (ga[c][k] * wl[c][k] - a[c][k] * m) : 0.f;
+            dz[k] = inside ? r * (gz[c][k] * wh[c][k] - z[c][k] * m) : 0.f;
+          }
+          if (act && on[c]) {
+            store<T, VEC>(ot + (long long)h * p.D + lo[c], da);
+            store<T, VEC>(ot + (long long)h * p.D + hi[c], dz);
+          }
+        }
+      }
+    }
+  }
+
+  if (BWD && sd.dw_partial) {
+    // the groups of a warp, then the warps, in a fixed order: the same inputs give the same bits
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        float u = dl[c][k], v = dh[c][k];
+        for (int o = G; o < 32; o <<= 1) {
+          u += __shfl_xor_sync(0xffffffffu, u, o);
+          v += __shfl_xor_sync(0xffffffffu, v, o);
+        }
+        if (lane < G && on[c]) {
+          sh_dw[warp * p.D + lo[c] + k] = u;
+          sh_dw[warp * p.D + hi[c] + k] = v;
+        }
+      }
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < p.D; d += kThreads) {
+      float s = 0.f;
+      for (int w = 0; w < kThreads / 32; ++w) s += sh_dw[w * p.D + d];
+      sd.dw_partial[(long long)block * p.D + d] = s;
+    }
+  }
+}
+
+// dw[d] = sum over blocks of partial[block][d], in a fixed order; grid.y: queries, keys
+__global__ void __launch_bounds__(256) qk_dweight_kernel(const float* pq, int nq, void* dq, int dtq, const float* pk, int nk, void* dk,
+                                                         int dtk, int D) {
+  __shared__ float sh[8][32];
+  const float* part = blockIdx.y ? pk : pq;
+  const int n = blockIdx.y ? nk : nq, dt = blockIdx.y ? dtk : dtq;
+  void* out = blockIdx.y ? dk : dq;
+  if (!out) return;
+  const int d = blockIdx.x * 32 + (threadIdx.x & 31), row = threadIdx.x >> 5;
+  float s = 0.f;
+  if (d < D)
+    for (int i = row; i < n; i += 8) s += part[(long long)i * D + d];
+  sh[row][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (row == 0 && d < D) {
+    s = 0.f;
+    for (int w = 0; w < 8; ++w) s += sh[w][threadIdx.x & 31];
+    if (dt == B200_F32) static_cast<float*>(out)[d] = s;
+    else if (dt == B200_BF16) static_cast<__nv_bfloat16*>(out)[d] = __float2bfloat16(s);
+    else static_cast<__half*>(out)[d] = __float2half(s);
+  }
+}
+
+// The widest vector (at most 16 bytes) that divides the halves, the heads and every stride and address.
+int vector_width(const B200QkNormRotary& p, bool bwd) {
+  const int es = p.dtype == B200_F32 ? 4 : 2;
+  for (int v = 16 / es; v > 1; v >>= 1) {
+    bool ok = p.D % (2 * v) == 0 && (p.interleaved ? p.R % (2 * v) == 0 : (p.R % (2 * v) == 0 && (p.D - p.R) % (2 * v) == 0));
+    for (int s = 0; ok && s < 2; ++s) {
+      const B200QkSide& q = p.side[s];
+      for (int i = 0; i < 3; ++i) ok = ok && q.x_stride[i] % v == 0 && (!bwd || q.dy_stride[i] % v == 0);
+      ok = ok && (uintptr_t)q.x % (v * es) == 0 && (uintptr_t)q.out % (v * es) == 0 && (!bwd || (uintptr_t)q.dy % (v * es) == 0);
+    }
+    if (ok) return v;
+  }
+  return 1;
+}
+
+int power_of_two_at_least(int n, int most) {
+  int g = 1;
+  while (g < n && g < most) g <<= 1;
+  return g;
+}
+
+struct Plan {
+  Args a;
+  int vec, ch, grid;
+};
+
+// The same plan for the launch and for the workspace size.
+Plan make_plan(const B200QkNormRotary& p, bool bwd) {
+  Plan pl{};
+  Args& a = pl.a;
+  pl.vec = vector_width(p, bwd);
+  const int units = p.D / (2 * pl.vec);
+  a.group = power_of_two_at_least(units, 32);
+  pl.ch = (units + a.group - 1) / a.group;
+  a.cos = p.cos; a.sin = p.sin; a.positions = p.positions; a.pos_b = p.pos_stride[0]; a.pos_l = p.pos_stride[1];
+  a.pos_is_64 = p.positions_dtype == B200_I64; a.table_rows = p.table_rows; a.bad_flag = p.bad_flag;
+  a.L = (unsigned)p.L; a.D = p.D; a.R = p.R; a.eps = p.eps;
+  const long long tokens = p.B * p.L;
+  for (int s = 0; s < 2; ++s) {
+    const B200QkSide& q = p.side[s];
+    Side& d = a.side[s];
+    d.x = q.x; d.dy = q.dy; d.out = q.out; d.weight = q.weight; d.weight_dtype = q.weight_dtype; d.heads = q.heads;
+    d.xs_b = q.x_stride[0]; d.xs_l = q.x_stride[1]; d.xs_h = q.x_stride[2];
+    d.gs_b = q.dy_stride[0]; d.gs_l = q.dy_stride[1]; d.gs_h = q.dy_stride[2];
+    // heads per item: as many as keep every SM busy with about 1024 threads, at most eight
+    int hpi = 1;
+    while (hpi < 8 && hpi * 2 <= q.heads && tokens * (q.heads / (hpi * 2)) * a.group >= 148LL * 1024) hpi *= 2;
+    d.heads_per_item = hpi;
+    d.items_per_token = (q.heads + hpi - 1) / hpi;
+    d.items = (unsigned)(tokens * d.items_per_token);
+    const long long per_block = kThreads / a.group;
+    long long blocks = (d.items + per_block - 1) / per_block;
+    const long long most = bwd ? 148 * 4 : 148 * 64;
+    d.blocks = (int)(blocks < most ? blocks : most);
+    pl.grid += d.blocks;
+  }
+  return pl;
+}
+
+template <typename T, int VEC, int CH, bool BWD>
+void launch(const Plan& pl, bool interleaved, cudaStream_t s) {
+  const size_t smem = BWD ? (size_t)(kThreads / 32) * pl.a.D * sizeof(float) : 0;
+  if (interleaved) qk_norm_rotary_kernel<T, VEC, CH, true, BWD><<<pl.grid, kThreads, smem, s>>>(pl.a);
+  else qk_norm_rotary_kernel<T, VEC, CH, false, BWD><<<pl.grid, kThreads, smem, s>>>(pl.a);
+}
+template <typename T, int WIDEST, bool BWD>
+int dispatch(const Plan& pl, bool interleaved, cudaStream_t s) {
+  // units of one head: D / (2 VEC) over at most 32 lanes, D at most 512
+  if (pl.vec == 8 && WIDEST == 8) launch<T, WIDEST == 8 ? 8 : 4, 1, BWD>(pl, interleaved, s);
+  else if (pl.vec == 4 && pl.ch == 1) launch<T, 4, 1, BWD>(pl, interleaved, s);
+  else if (pl.vec == 4) launch<T, 4, 2, BWD>(pl, interleaved, s);
+  else if (pl.vec == 2 && pl.ch == 1) launch<T, 2, 1, BWD>(pl, interleaved, s);
+  else if (pl.vec == 2) launch<T, 2, 4, BWD>(pl, interleaved, s);
+  else if (pl.ch == 1) launch<T, 1, 1, BWD>(pl, interleaved, s);
+  else launch<T, 1, 8, BWD>(pl, interleaved, s);
+  return (int)cudaGetLastError();
+}
+
+bool valid(const B200QkNormRotary* p) {
+  if (p->D <= 0 || p->D % 2 || p->D > B200_QK_MAX_HEAD_DIM || p->R < 0 || p->R % 2 || p->R > p->D) return false;
+  for (int s = 0; s < 2; ++s)
+    if (p->side[s].heads < 0 || p->B * p->L * (long long)p->side[s].heads >= (1LL << 31)) return false;
+  return true;
+}
+
+}  // namespace
+
+extern "C" long long b200_qk_norm_rotary_workspace(const B200QkNormRotary* p) {
+  if (!valid(p) || p->B * p->L <= 0) return 0;
+  return (long long)make_plan(*p, true).grid * p->D * sizeof(float);
+}
+
+extern "C" int b200_qk_norm_rotary_fwd(const B200QkNormRotary* p, void* stream) {
+  if (!valid(p)) return (int)cudaErrorInvalidValue;
+  if (p->B * p->L <= 0) return 0;
+  const Plan pl = make_plan(*p, false);
+  if (pl.grid == 0) return 0;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (p->dtype == B200_BF16) return dispatch<__nv_bfloat16, 8, false>(pl, p->interleaved, s);
+  if (p->dtype == B200_F16) return dispatch<__half, 8, false>(pl, p->interleaved, s);
+  if (p->dtype == B200_F32) return dispatch<float, 4, false>(pl, p->interleaved, s);
+  return (int)cudaErrorInvalidValue;
+}
+
+extern "C" int b200_qk_norm_rotary_bwd(const B200QkNormRotary* p, void* workspace, void* stream) {
+  if (!valid(p)) return (int)cudaErrorInvalidValue;
+  cudaStream_t s = (cudaStream_t)stream;
+  Plan pl = p->B * p->L > 0 ? make_plan(*p, true) : Plan{};
+  float* ws = static_cast<float*>(workspace);
+  for (int i = 0; i < 2; ++i) {
+    if (p->side[i].dweight) pl.a.side[i].dw_partial = ws;
+    ws += (long long)pl.a.side[i].blocks * p->D;
+  }
+  if (pl.grid > 0) {
+    int rc;
+    if (p->dtype == B200_BF16) rc = dispatch<__nv_bfloat16, 8, true>(pl, p->interleaved, s);
+    else if (p->dtype == B200_F16) rc = dispatch<__half, 8, true>(pl, p->interleaved, s);
+    else if (p->dtype == B200_F32) rc = dispatch<float, 4, true>(pl, p->interleaved, s);
+    else rc = (int)cudaErrorInvalidValue;
+    if (rc) return rc;
+  }
+  if (p->side[0].dweight || p->side[1].dweight) {
+    qk_dweight_kernel<<<dim3((p->D + 31) / 32, 2), 256, 0, s>>>(
+        pl.a.side[0].dw_partial, pl.a.side[0].blocks, p->side[0].dweight, p->side[0].weight_dtype, pl.a.side[1].dw_partial,
+        pl.a.side[1].blocks, p->side[1].dweight, p->side[1].weight_dtype, p->D);
+  }
+  return (int)cudaGetLastError();
+}

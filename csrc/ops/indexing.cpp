@@ -49,6 +49,15 @@ void check_bad_index(const char* op, int device) {
 }
 int* bad_ptr(const Tensor& like) { return bad_index_flag(like.device().index()).data_ptr<int>(); }
 
+
+}  // namespace
+
+// For operators elsewhere: the flag is read in synchronous mode only, so only then is there one to set.
+int* checked_index_flag(const at::Tensor& like) { return flags().async_disable ? bad_ptr(like) : nullptr; }
+void report_bad_index(const char* op, const at::Tensor& like) { check_bad_index(op, like.device().index()); }
+
+namespace {
+
 std::vector<long long> ll(at::IntArrayRef v) { return std::vector<long long>(v.begin(), v.end()); }
 
 // ---- gather / scatter ----------------------------------------------------------------

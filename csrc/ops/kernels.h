@@ -49,5 +49,10 @@ void launch_ew(at::TensorIteratorBase& iter, int op, double s0, double s1, void*
 void launch_copy(const at::Tensor& src, const at::Tensor& dst, void* stream);
 void launch_fill(const at::Tensor& dst, double value, void* stream);
 
+// The device flag that a kernel sets when it meets an index out of range (the access is skipped): null unless the
+// backend runs in synchronous mode, where report_bad_index raises an IndexError and clears it after the launch.
+int* checked_index_flag(const at::Tensor& like);
+void report_bad_index(const char* op, const at::Tensor& like);
+
 }  // namespace ops
 }  // namespace catch_b200

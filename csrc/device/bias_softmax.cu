@@ -444,26 +444,32 @@ __global__ void __launch_bounds__(kMaxThreads) bias_softmax_bwd_long(const __gri
   for (int x = threadIdx.x; x <= last; x += blockDim.x) out[x] = acc[padded(x)];
 }
 
-// One block per head: sums over blocks for each distance, then over the distances of each bucket, in a fixed order.
+// One block per head and bucket: sums over the blocks' partial sums for the distances of the bucket, in a fixed order.  A
+// bucket's distances are neighbours, so its slots are one run [x0, x1].
 __global__ void __launch_bounds__(kMaxThreads) bias_table_grad(const float* partial, int blocks, int reach, const __grid_constant__ B200RelativeBuckets rb,
                                                                int H, void* out, int dtype) {
-  extern __shared__ float diag[];
-  const int h = blockIdx.x, last = 2 * reach;
-  const float* mine = partial + (long long)h * blocks * (last + 1);
-  for (int x = threadIdx.x; x <= last; x += blockDim.x) {
-    float t = 0.f;
-    for (int b = 0; b < blocks; ++b) t += mine[(long long)b * (last + 1) + x];
-    diag[x] = t;
+  __shared__ float sh[32];
+  const int h = blockIdx.x, bucket = blockIdx.y, slots = 2 * reach + 1;
+  const bool upper = rb.bidirectional && bucket >= rb.per_side;
+  const int c = upper ? bucket - rb.per_side : bucket, far = c - rb.exact;
+  int lo = far >= 0 ? rb.first[far] : c;
+  int hi = c == rb.per_side - 1 ? reach : (far >= 0 ? rb.first[far + 1] : c + 1) - 1;
+  if (upper && lo == 0) lo = 1;  // distance 0 belongs to the lower half
+  hi = min(hi, reach);
+  int x0 = upper ? reach + lo : reach - hi, x1 = upper ? reach + hi : reach - lo;
+  if (!rb.bidirectional && c == 0) x1 = 2 * reach;  // keys after the query
+  float t = 0.f;
+  if (lo <= hi) {
+    const float* mine = partial + (long long)h * blocks * slots + x0;
+    const unsigned run = (unsigned)(x1 - x0 + 1), n = run * (unsigned)blocks;
+    for (unsigned i = threadIdx.x; i < n; i += blockDim.x) t += mine[(long long)(i / run) * slots + i % run];
   }
-  __syncthreads();
-  const int buckets = rb.bidirectional ? 2 * rb.per_side : rb.per_side;
-  for (int b = threadIdx.x; b < buckets; b += blockDim.x) {
-    float t = 0.f;
-    for (int x = 0; x <= last; ++x)
-      if (bucket_of(x - reach, rb) == b) t += diag[x];
-    if (dtype == B200_F32) static_cast<float*>(out)[(long long)b * H + h] = t;
-    else if (dtype == B200_BF16) static_cast<__nv_bfloat16*>(out)[(long long)b * H + h] = __float2bfloat16(t);
-    else static_cast<__half*>(out)[(long long)b * H + h] = __float2half(t);
+  t = block_sum(t, sh);
+  if (threadIdx.x == 0) {
+    const long long at = (long long)bucket * H + h;
+    if (dtype == B200_F32) static_cast<float*>(out)[at] = t;
+    else if (dtype == B200_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16(t);
+    else static_cast<__half*>(out)[at] = __float2half(t);
   }
 }
 
@@ -581,12 +587,8 @@ extern "C" int b200_bias_softmax_bwd(const B200BiasSoftmax* p, void* workspace, 
   pl.a.partial = p->dtable ? static_cast<float*>(workspace) : nullptr;
   const int rc = dispatch_type(pl, p->dtype, true, s);
   if (rc || !p->dtable) return rc;
-  const size_t smem = (size_t)(2 * pl.a.reach + 1) * 4;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute((const void*)bias_table_grad, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-  }
-  bias_table_grad<<<(unsigned)p->H, kMaxThreads, smem, s>>>(pl.a.partial, pl.a.blocks_per_head, pl.a.reach, p->buckets, p->H, p->dtable,
-                                                            p->table_dtype);
+  const int buckets = p->buckets.per_side * (p->buckets.bidirectional ? 2 : 1);
+  bias_table_grad<<<dim3((unsigned)p->H, (unsigned)buckets), kMaxThreads, 0, s>>>(pl.a.partial, pl.a.blocks_per_head, pl.a.reach, p->buckets, p->H,
+                                                                                p->dtable, p->table_dtype);
   return (int)cudaGetLastError();
 }

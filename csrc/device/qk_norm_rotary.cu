@@ -247,26 +247,29 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rotary_kernel(const __grid_c
   }
 }
 
-// dw[d] = sum over blocks of partial[block][d], in a fixed order; grid.y: queries, keys
-__global__ void __launch_bounds__(256) qk_dweight_kernel(const float* pq, int nq, void* dq, int dtq, const float* pk, int nk, void* dk,
-                                                         int dtk, int D) {
-  __shared__ float sh[8][32];
+// dw[d] = sum over blocks of partial[block][d], in a fixed order; grid.y: queries, keys.  Some hundred rows of partial sums: 32 of
+// them side by side with several loads under way, since this is latency and nothing else.
+__global__ void __launch_bounds__(1024) qk_dweight_kernel(const float* pq, int nq, void* dq, int dtq, const float* pk, int nk, void* dk,
+                                                          int dtk, int D) {
+  __shared__ float sh[32][33];
   const float* part = blockIdx.y ? pk : pq;
   const int n = blockIdx.y ? nk : nq, dt = blockIdx.y ? dtk : dtq;
   void* out = blockIdx.y ? dk : dq;
   if (!out) return;
-  const int d = blockIdx.x * 32 + (threadIdx.x & 31), row = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, d = blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (d < D)
-    for (int i = row; i < n; i += 8) s += part[(long long)i * D + d];
-  sh[row][threadIdx.x & 31] = s;
+  if (d < D) {
+#pragma unroll 8
+    for (int i = row; i < n; i += 32) s += part[(long long)i * D + d];
+  }
+  sh[row][lane] = s;
   __syncthreads();
-  if (row == 0 && d < D) {
-    s = 0.f;
-    for (int w = 0; w < 8; ++w) s += sh[w][threadIdx.x & 31];
-    if (dt == B200_F32) static_cast<float*>(out)[d] = s;
-    else if (dt == B200_BF16) static_cast<__nv_bfloat16*>(out)[d] = __float2bfloat16(s);
-    else static_cast<__half*>(out)[d] = __float2half(s);
+  s = group_sum(sh[lane][row], 32);  // warp `row` adds column `row`
+  const int e = blockIdx.x * 32 + row;
+  if (lane == 0 && e < D) {
+    if (dt == B200_F32) static_cast<float*>(out)[e] = s;
+    else if (dt == B200_BF16) static_cast<__nv_bfloat16*>(out)[e] = __float2bfloat16(s);
+    else static_cast<__half*>(out)[e] = __float2half(s);
   }
 }
 
@@ -392,7 +395,7 @@ extern "C" int b200_qk_norm_rotary_bwd(const B200QkNormRotary* p, void* workspac
     if (rc) return rc;
   }
   if (p->side[0].dweight || p->side[1].dweight) {
-    qk_dweight_kernel<<<dim3((p->D + 31) / 32, 2), 256, 0, s>>>(
+    qk_dweight_kernel<<<dim3((p->D + 31) / 32, 2), 1024, 0, s>>>(
         pl.a.side[0].dw_partial, pl.a.side[0].blocks, p->side[0].dweight, p->side[0].weight_dtype, pl.a.side[1].dw_partial,
         pl.a.side[1].blocks, p->side[1].dweight, p->side[1].weight_dtype, p->D);
   }

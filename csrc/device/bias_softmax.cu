@@ -33,7 +33,8 @@ struct Args {
   long long st_b, st_h, st_i;     // of s, g and out (their last dimension is dense)
   long long mk_b, mk_h, mk_i, mk_j;
   int table_dtype, mask_dtype;
-  int H, Lq, Lk, reach, offset;
+  int H, Lq, Lk, offset;
+  int reach, last;      // distances -reach .. last - reach have a slot each, farther ones the slot at their end
   unsigned rows;        // of one head: B * Lq
   unsigned rows_per_block;
   int blocks_per_head, group;
@@ -61,270 +62,300 @@ __device__ __forceinline__ int bucket_of(int rel, const B200RelativeBuckets& rb)
 }
 
 // One pad word every 32: lanes that read eight neighbours each then meet in different banks.
-__device__ __forceinline__ int padded(int x) { return x + (x >> 5); }
+__host__ __device__ __forceinline__ int padded(int x) { return x + (x >> 5); }
 
 __device__ __forceinline__ void fill_lut(float* lut, const Args& p, int h) {
-  for (int x = threadIdx.x; x <= 2 * p.reach; x += blockDim.x)
+  for (int x = threadIdx.x; x <= p.last; x += blockDim.x)
     lut[padded(x)] = scalar_at(p.table, (long long)bucket_of(x - p.reach, p.rb) * p.H + h, p.table_dtype);
 }
 
-// The elements [j0, j0 + VEC) of a row; those outside [0, n) are left alone.  A vector lies on a 16-byte boundary.
-template <typename T, int VEC>
-__device__ __forceinline__ void load_part(const T* row, int j0, int n, float (&v)[VEC]) {
-  if (j0 >= 0 && j0 + VEC <= n) {
-    load<T, VEC>(row + j0, v);
-  } else {
+// Vectors of VEC elements (16 bytes) on 16-byte boundaries.  EDGE: rows may begin anywhere and have any length, so that the
+// first and the last vector can reach over the row's ends; without it (rows begin on boundaries and have whole vectors) those tests are gone.
+// The elements [j0, j0 + VEC) of a row; those outside [0, n) read as 0 and are not written.
+template <typename T, int VEC, bool EDGE>
+__device__ __forceinline__ Pack<T, VEC> load_part(const T* row, int j0, int n) {
+  if (!EDGE || (j0 >= 0 && j0 + VEC <= n)) return *reinterpret_cast<const Pack<T, VEC>*>(row + j0);
+  Pack<T, VEC> v;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) v[k] = j0 + k >= 0 && j0 + k < n ? to_f32<T>(row[j0 + k]) : 0.f;
-  }
+  for (int k = 0; k < VEC; ++k) v.v[k] = j0 + k >= 0 && j0 + k < n ? row[j0 + k] : from_f32<T>(0.f);
+  return v;
 }
-template <typename T, int VEC>
-__device__ __forceinline__ void store_part(T* row, int j0, int n, const float (&v)[VEC]) {
-  if (j0 >= 0 && j0 + VEC <= n) {
-    store<T, VEC>(row + j0, v);
+template <typename T, int VEC, bool EDGE>
+__device__ __forceinline__ void store_part(T* row, int j0, int n, const Pack<T, VEC>& v) {
+  if (!EDGE || (j0 >= 0 && j0 + VEC <= n)) {
+    *reinterpret_cast<Pack<T, VEC>*>(row + j0) = v;
   } else {
 #pragma unroll
     for (int k = 0; k < VEC; ++k)
-      if (j0 + k >= 0 && j0 + k < n) row[j0 + k] = from_f32<T>(v[k]);
+      if (j0 + k >= 0 && j0 + k < n) row[j0 + k] = v.v[k];
   }
 }
 
+__device__ __forceinline__ float2 masked(float2 a, float2 m) {
+  return make_float2(m.x == kNegInf ? kNegInf : a.x + m.x, m.y == kNegInf ? kNegInf : a.y + m.y);
+}
 template <typename M, int VEC>
-__device__ __forceinline__ void add_mask_vector(const M* m, float (&a)[VEC]) {
-  float v[VEC];
+__device__ __forceinline__ void add_mask_vector(const M* m, float2 (&a)[VEC / 2]) {
   constexpr int W = 16 / sizeof(M) < VEC ? 16 / sizeof(M) : VEC;
 #pragma unroll
   for (int o = 0; o < VEC; o += W) {
-    float part[W];
-    load<M, W>(m + o, part);
+    const Pack<M, W> part = *reinterpret_cast<const Pack<M, W>*>(m + o);
 #pragma unroll
-    for (int k = 0; k < W; ++k) v[o + k] = part[k];
+    for (int k = 0; k < W / 2; ++k) a[o / 2 + k] = masked(a[o / 2 + k], pair_of(part, k));
   }
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) a[k] = v[k] == kNegInf ? kNegInf : a[k] + v[k];
+}
+
+// The mask of one row: where key 0 has its element, and whether the row's vectors lie on the boundaries of wide loads.
+struct MaskRow {
+  const char* key0;
+  bool wide;
+};
+__device__ __forceinline__ int mask_bytes(int dtype) { return dtype == B200_F32 ? 4 : (dtype == B200_BF16 || dtype == B200_F16 ? 2 : 1); }
+template <int VEC>
+__device__ __forceinline__ MaskRow mask_row(const Args& p, long long at, int phase) {
+  const int es = mask_bytes(p.mask_dtype);
+  MaskRow m;
+  m.key0 = static_cast<const char*>(p.mask) + at * es;
+  m.wide = p.mk_j == 1 && ((reinterpret_cast<uintptr_t>(m.key0) - phase * es) & ((VEC * es < 16 ? VEC * es : 16) - 1)) == 0;
+  return m;
 }
 
 // Adds the mask to the scores of [j0, j0 + VEC); excluded elements become -inf whatever they held, NaN too.
-template <int VEC>
-__device__ __forceinline__ void add_mask(const Args& p, long long row, int j0, float (&a)[VEC]) {
-  const long long at = row + (long long)j0 * p.mk_j;
-  if (p.mk_j == 1 && j0 >= 0 && j0 + VEC <= p.Lk) {
-    const int es = p.mask_dtype == B200_F32 ? 4 : (p.mask_dtype == B200_BF16 || p.mask_dtype == B200_F16 ? 2 : 1);
-    const char* m = static_cast<const char*>(p.mask) + at * es;
-    const int bytes = VEC * es < 16 ? VEC * es : 16;
-    if ((reinterpret_cast<uintptr_t>(m) & (bytes - 1)) == 0) {
-      if (es == 4) { add_mask_vector<float, VEC>(reinterpret_cast<const float*>(m), a); return; }
-      if (p.mask_dtype == B200_BF16) { add_mask_vector<__nv_bfloat16, VEC>(reinterpret_cast<const __nv_bfloat16*>(m), a); return; }
-      if (p.mask_dtype == B200_F16) { add_mask_vector<__half, VEC>(reinterpret_cast<const __half*>(m), a); return; }
+template <int VEC, bool EDGE>
+__device__ __forceinline__ void add_mask(const Args& p, const MaskRow& row, int j0, float2 (&a)[VEC / 2]) {
+  if (row.wide && (!EDGE || (j0 >= 0 && j0 + VEC <= p.Lk))) {
+    const char* m = row.key0 + j0 * mask_bytes(p.mask_dtype);
+    if (p.mask_dtype == B200_F32) add_mask_vector<float, VEC>(reinterpret_cast<const float*>(m), a);
+    else if (p.mask_dtype == B200_BF16) add_mask_vector<__nv_bfloat16, VEC>(reinterpret_cast<const __nv_bfloat16*>(m), a);
+    else if (p.mask_dtype == B200_F16) add_mask_vector<__half, VEC>(reinterpret_cast<const __half*>(m), a);
+    else {
       const Pack<unsigned char, VEC> keep = *reinterpret_cast<const Pack<unsigned char, VEC>*>(m);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) a[k] = keep.v[k] ? a[k] : kNegInf;
-      return;
+      for (int k = 0; k < VEC / 2; ++k) a[k] = make_float2(keep.v[2 * k] ? a[k].x : kNegInf, keep.v[2 * k + 1] ? a[k].y : kNegInf);
     }
-  }
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) {
-    if (j0 + k >= 0 && j0 + k < p.Lk) {
-      const float v = scalar_at(p.mask, at + k * p.mk_j, p.mask_dtype);
-      a[k] = v == kNegInf ? kNegInf : a[k] + v;
-    }
-  }
-}
-
-// Scores to logits: scale, bias by distance, mask; -inf outside the row.  x0 = distance of the first element + reach.
-template <int VEC>
-__device__ __forceinline__ void to_logits(const Args& p, const float* lut, long long mask_row, int j0, int x0, float (&a)[VEC]) {
-  const int last = 2 * p.reach;
-  if (x0 >= last || x0 + VEC - 1 <= 0) {  // all as far as the bias tells apart
-    const float b = lut[padded(x0 > 0 ? last : 0)];
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) a[k] = fmaf(a[k], p.scale, b);
-  } else {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) a[k] = fmaf(a[k], p.scale, lut[padded(min(max(x0 + k, 0), last))]);
-  }
-  if (p.mask) add_mask<VEC>(p, mask_row, j0, a);
-  if (j0 < 0 || j0 + VEC > p.Lk) {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k)
-      if (j0 + k < 0 || j0 + k >= p.Lk) a[k] = kNegInf;
-  }
-}
-
-__device__ __forceinline__ float weight_of(float a, float m) { return a == kNegInf ? 0.f : __expf(a - m); }
-
-// d to the table gradient's sums over distances
-template <int VEC>
-__device__ __forceinline__ void add_distances(float* acc, int last, int x0, const float (&d)[VEC], float& below, float& above) {
-  if (x0 >= last || x0 + VEC - 1 <= 0) {
-    float t = 0.f;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) t += d[k];
-    if (x0 > 0) above += t; else below += t;
     return;
   }
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) {
-    const int x = x0 + k;
-    if (x <= 0) below += d[k];
-    else if (x >= last) above += d[k];
-    else acc[padded(x)] += d[k];
+  for (int k = 0; k < VEC / 2; ++k) {
+    const int j = j0 + 2 * k;
+    float2 m = make_float2(0.f, 0.f);
+    if (j >= 0 && j < p.Lk) m.x = scalar_at(row.key0, j * p.mk_j, p.mask_dtype);
+    if (j + 1 >= 0 && j + 1 < p.Lk) m.y = scalar_at(row.key0, (j + 1) * p.mk_j, p.mask_dtype);
+    a[k] = masked(a[k], m);
   }
 }
 
-struct RowAt {
-  long long at, mask_row;
-  long long stat;
-  int first_x;  // distance of key 0 plus reach
-};
-__device__ __forceinline__ RowAt row_at(const Args& p, unsigned r, int h) {
-  const unsigned b = r / (unsigned)p.Lq, i = r % (unsigned)p.Lq;
-  RowAt w;
-  w.at = b * p.st_b + h * p.st_h + i * p.st_i;
-  w.mask_row = b * p.mk_b + h * p.mk_h + i * p.mk_i;
-  w.stat = ((long long)b * p.H + h) * p.Lq + i;
-  w.first_x = p.reach - p.offset - (int)i;
-  return w;
+// Scores to logits: scale, bias by distance, mask; -inf outside the row.  x0 = slot of the first element's distance.
+template <typename T, int VEC, bool MASKED, bool EDGE>
+__device__ __forceinline__ void to_logits(const Args& p, const float* lut, const MaskRow& mask, int j0, int x0, const Pack<T, VEC>& s, float2 (&a)[VEC / 2]) {
+  const int last = p.last;
+  const float2 scale = both(p.scale);
+  if (x0 >= last || x0 + VEC - 1 <= 0) {  // all as far as the bias tells apart
+    const float2 b = both(lut[x0 > 0 ? padded(last) : 0]);
+#pragma unroll
+    for (int k = 0; k < VEC / 2; ++k) a[k] = fma2(pair_of(s, k), scale, b);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC / 2; ++k) {
+      const int x = x0 + 2 * k;
+      a[k] = fma2(pair_of(s, k), scale, make_float2(lut[padded(min(max(x, 0), last))], lut[padded(min(max(x + 1, 0), last))]));
+    }
+  }
+  if (MASKED) add_mask<VEC, EDGE>(p, mask, j0, a);
+  if (EDGE && (j0 < 0 || j0 + VEC > p.Lk)) {
+#pragma unroll
+    for (int k = 0; k < VEC / 2; ++k) {
+      const int j = j0 + 2 * k;
+      if (j < 0 || j >= p.Lk) a[k].x = kNegInf;
+      if (j + 1 < 0 || j + 1 >= p.Lk) a[k].y = kNegInf;
+    }
+  }
 }
 
-// A row to a group of lanes, in registers: NV vectors of VEC elements for each lane.
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(kMaxThreads) bias_softmax_fwd_rows(const __grid_constant__ Args p) {
+// e^(a - m).  The difference comes first: a and m may be as large as the type allows (a mask of its lowest value on a whole row).
+// a = -inf gives 0 as long as m is finite, see finite_max.
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float weight_of(float a, float m) { return exp2_fast((a - m) * kLog2e); }
+__device__ __forceinline__ float2 weights_of(float2 a, float2 minus_m) {
+  const float2 t = mul2(add2(a, minus_m), both(kLog2e));
+  return make_float2(exp2_fast(t.x), exp2_fast(t.y));
+}
+__device__ __forceinline__ float finite_max(float m) { return m == kNegInf ? 0.f : m; }
+// 1 / sum, 0 for a row with nothing left (a NaN stays one)
+__device__ __forceinline__ float inverse_sum(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+template <int N>
+__device__ __forceinline__ float max_of(float m, const float2 (&a)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) m = fmaxf(m, fmaxf(a[k].x, a[k].y));
+  return m;
+}
+
+// d to the table gradient's sums over distances
+template <int VEC>
+__device__ __forceinline__ void add_distances(float* acc, int last, int x0, const float2 (&d)[VEC / 2], float& below, float& above) {
+  if (x0 >= last || x0 + VEC - 1 <= 0) {
+    float2 t = d[0];
+#pragma unroll
+    for (int k = 1; k < VEC / 2; ++k) t = add2(t, d[k]);
+    if (x0 > 0) above += t.x + t.y; else below += t.x + t.y;
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const int x = x0 + k;
+      const float v = k % 2 ? d[k / 2].y : d[k / 2].x;
+      if (x <= 0) below += v;
+      else if (x >= last) above += v;
+      else acc[padded(x)] += v;
+    }
+  }
+}
+
+// Walks over the rows (b, i) of a head.
+struct RowWalk {
+  unsigned i;
+  int h;
+  long long at, mask, stat;  // where the row's scores, mask and statistics begin
+  __device__ __forceinline__ RowWalk(const Args& p, unsigned r, int head) : i(r % (unsigned)p.Lq), h(head) {
+    const unsigned b = r / (unsigned)p.Lq;
+    at = b * p.st_b + h * p.st_h + i * p.st_i;
+    mask = b * p.mk_b + h * p.mk_h + i * p.mk_i;
+    stat = ((long long)b * p.H + h) * p.Lq + i;
+  }
+  __device__ __forceinline__ void advance(const Args& p, unsigned step) {
+    i += step;
+    at += step * p.st_i;
+    mask += step * p.mk_i;
+    stat += step;
+    while (i >= (unsigned)p.Lq) {
+      i -= (unsigned)p.Lq;
+      at += p.st_b - p.Lq * p.st_i;
+      mask += p.mk_b - p.Lq * p.mk_i;
+      stat += (long long)(p.H - 1) * p.Lq;
+    }
+  }
+  __device__ __forceinline__ int first_x(const Args& p) const { return p.reach - p.offset - (int)i; }  // slot of key 0's distance
+};
+
+// (maximum, sum) of the lanes of one row.  WARPS = 1: the row belongs to a group of G lanes.  WARPS > 1: to the block, whose warps
+// meet once in shared memory, in one of two places in turn, so that one barrier a row is enough.
+template <int WARPS>
+__device__ __forceinline__ float2 join_rows(float m, float sum, int G, float2 (*sh)[WARPS], int turn) {
+  if (WARPS == 1) return make_float2(m, sum);  // m is the group's already
+  if ((threadIdx.x & 31) == 0) sh[turn][threadIdx.x >> 5] = make_float2(m, sum);
+  __syncthreads();
+  float top = kNegInf, all = 0.f;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sh[turn][w].x);
+  const float t = finite_max(top);
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    const float2 o = sh[turn][w];
+    all += o.y * weight_of(o.x, t);  // a warp without keys: 0 times 0; one with a NaN score: NaN
+  }
+  return make_float2(top, all);
+}
+
+// Registers: 64 a thread forward and 80 backward hold 16 elements of a lane and leave 1024 and 768 threads for an SM.  Left alone, the
+// compiler takes 120 for the loads of a mask whose keys are not side by side, which is the rare case.
+constexpr int row_threads(int warps) { return warps == 1 ? kMaxThreads : 32 * warps; }
+constexpr int row_blocks(int elements, int warps, int resident) { return elements <= 16 ? resident / row_threads(warps) : 1; }
+
+// A row in registers: NV vectors of VEC elements for each of its lanes (a group of G of one warp, or the block's WARPS warps).
+template <typename T, int VEC, int NV, int WARPS, bool MASKED, bool EDGE>
+__global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS, 1024)) bias_softmax_fwd_rows(const __grid_constant__ Args p) {
   extern __shared__ float lut[];
+  __shared__ float2 meet[2][WARPS];
   const int h = blockIdx.x / p.blocks_per_head, part = blockIdx.x % p.blocks_per_head;
   fill_lut(lut, p, h);
   __syncthreads();
-  const int G = p.group, gl = threadIdx.x & (G - 1), groups = blockDim.x / G;
+  const int G = WARPS == 1 ? p.group : 32, lanes = G * WARPS;
+  const int gl = WARPS == 1 ? threadIdx.x & (G - 1) : threadIdx.x, groups = WARPS == 1 ? blockDim.x / G : 1;
   const unsigned r0 = part * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
-  for (unsigned base = r0; base < r1; base += groups) {
-    const unsigned r = base + threadIdx.x / G;
-    const bool live = r < r1;
-    const RowAt w = row_at(p, live ? r : r0, h);
-    const T* s = static_cast<const T*>(p.s) + w.at;
-    const int phase = (int)((reinterpret_cast<uintptr_t>(s) / sizeof(T)) & (VEC - 1));
-    float a[NV][VEC], m = kNegInf;
+  const unsigned r = WARPS == 1 ? r0 + threadIdx.x / G : r0;
+  RowWalk walk(p, min(r, p.rows - 1), h);  // a group behind the last row follows on rows that are there
+  int turn = 0;
+  for (unsigned done = 0; r0 + done < r1; done += groups, turn ^= 1) {
+    const bool live = r + done < r1;
+    const T* s = static_cast<const T*>(p.s) + walk.at;
+    const int phase = EDGE ? (int)((reinterpret_cast<uintptr_t>(s) / sizeof(T)) & (VEC - 1)) : 0;
+    const MaskRow mask = MASKED ? mask_row<VEC>(p, walk.mask, phase) : MaskRow{};
+    const int first_x = walk.first_x(p);
+    Pack<T, VEC> raw[NV];
+    float2 a[NV][VEC / 2];
+    float m = kNegInf;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int j0 = (gl + n * G) * VEC - phase;
-      if (j0 < p.Lk) load_part<T, VEC>(s, j0, p.Lk, a[n]);
+      const int j0 = (gl + n * lanes) * VEC - phase;
+      if (j0 < p.Lk) raw[n] = load_part<T, VEC, EDGE>(s, j0, p.Lk);
     }
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int j0 = (gl + n * G) * VEC - phase;
+      const int j0 = (gl + n * lanes) * VEC - phase;
       if (j0 < p.Lk) {
-        to_logits<VEC>(p, lut, w.mask_row, j0, w.first_x + j0, a[n]);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) m = fmaxf(m, a[n][k]);
+        to_logits<T, VEC, MASKED, EDGE>(p, lut, mask, j0, first_x + j0, raw[n], a[n]);
+        m = max_of(m, a[n]);
       }
     }
     m = group_max(m, G);
-    float sum = 0.f;
+    const float2 minus = both(-finite_max(m));
+    float2 sum2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      if ((gl + n * G) * VEC - phase < p.Lk) {
+      if ((gl + n * lanes) * VEC - phase < p.Lk) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          a[n][k] = weight_of(a[n][k], m);
-          sum += a[n][k];
+        for (int k = 0; k < VEC / 2; ++k) {
+          a[n][k] = weights_of(a[n][k], minus);
+          sum2 = add2(sum2, a[n][k]);
         }
       }
     }
-    sum = group_sum(sum, G);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (!live) continue;
-    T* o = static_cast<T*>(p.out) + w.at;
+    const float2 row = join_rows<WARPS>(m, group_sum(sum2.x + sum2.y, G), G, meet, turn);
+    const float inv = inverse_sum(row.y), f = WARPS == 1 ? inv : inv * weight_of(m, finite_max(row.x));
+    if (live) {
+      T* o = static_cast<T*>(p.out) + walk.at;
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int j0 = (gl + n * G) * VEC - phase;
-      if (j0 < p.Lk) {
+      for (int n = 0; n < NV; ++n) {
+        const int j0 = (gl + n * lanes) * VEC - phase;
+        if (j0 < p.Lk) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) a[n][k] *= inv;
-        store_part<T, VEC>(o, j0, p.Lk, a[n]);
+          for (int k = 0; k < VEC / 2; ++k) set_pair(raw[n], k, mul2(a[n][k], both(f)));
+          store_part<T, VEC, EDGE>(o, j0, p.Lk, raw[n]);
+        }
       }
+      if (p.stats && gl == 0) p.stats[walk.stat] = make_float2(finite_max(row.x), inv);
+      if (r + done + groups < r1) walk.advance(p, groups);
     }
-    if (p.stats && gl == 0) p.stats[w.stat] = make_float2(m, inv);
   }
 }
 
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(kMaxThreads) bias_softmax_bwd_rows(const __grid_constant__ Args p) {
-  extern __shared__ float lut[];
-  const int last = 2 * p.reach, words = padded(last) + 1;
-  const int h = blockIdx.x / p.blocks_per_head, part = blockIdx.x % p.blocks_per_head;
-  const int G = p.group, gl = threadIdx.x & (G - 1), groups = blockDim.x / G;
-  float* all = lut + words;
-  float* acc = all + (threadIdx.x / G) * words;
-  fill_lut(lut, p, h);
-  if (p.partial)
-    for (int x = threadIdx.x; x < groups * words; x += blockDim.x) all[x] = 0.f;
+template <int WARPS>
+__device__ __forceinline__ float join_sums(float v, float (*sh)[WARPS], int turn) {
+  if (WARPS == 1) return v;
+  if ((threadIdx.x & 31) == 0) sh[turn][threadIdx.x >> 5] = v;
   __syncthreads();
-  float below = 0.f, above = 0.f;
-  const unsigned r0 = part * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
-  for (unsigned base = r0; base < r1; base += groups) {
-    const unsigned r = base + threadIdx.x / G;
-    const bool live = r < r1;
-    const RowAt w = row_at(p, live ? r : r0, h);
-    const T* s = static_cast<const T*>(p.s) + w.at;
-    const T* g = static_cast<const T*>(p.g) + w.at;
-    const int phase = (int)((reinterpret_cast<uintptr_t>(s) / sizeof(T)) & (VEC - 1));
-    const float2 st = p.stats[w.stat];
-    float a[NV][VEC], d[NV][VEC], dot = 0.f;
+  float all = 0.f;
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int j0 = (gl + n * G) * VEC - phase;
-      if (j0 < p.Lk) {
-        load_part<T, VEC>(s, j0, p.Lk, a[n]);
-        load_part<T, VEC>(g, j0, p.Lk, d[n]);
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int j0 = (gl + n * G) * VEC - phase;
-      if (j0 < p.Lk) {
-        to_logits<VEC>(p, lut, w.mask_row, j0, w.first_x + j0, a[n]);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          a[n][k] = weight_of(a[n][k], st.x) * st.y;
-          dot += a[n][k] == 0.f ? 0.f : a[n][k] * d[n][k];  // an excluded key counts nothing, whatever its gradient holds
-        }
-      }
-    }
-    dot = group_sum(dot, G);
-    if (live) {
-      T* o = static_cast<T*>(p.out) + w.at;
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const int j0 = (gl + n * G) * VEC - phase;
-        if (j0 < p.Lk) {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) {
-            d[n][k] = a[n][k] == 0.f ? 0.f : a[n][k] * (d[n][k] - dot);
-            a[n][k] = d[n][k] * p.scale;
-          }
-          store_part<T, VEC>(o, j0, p.Lk, a[n]);
-          if (p.partial) add_distances<VEC>(acc, last, w.first_x + j0, d[n], below, above);
-        }
-      }
-    }
-    __syncwarp();  // the next row of this group adds to the same sums from other lanes
-  }
-  if (!p.partial) return;
-  below = group_sum(below, G);
-  above = group_sum(above, G);
-  if (gl == 0) {  // the slots of the two ends are used for nothing else
+  for (int w = 0; w < WARPS; ++w) all += sh[turn][w];
+  return all;
+}
+
+// The sums over distances of a block, to its place among the partial sums.
+__device__ __forceinline__ void write_partial(const Args& p, float* all, int groups, int words, float* acc, int h, int part, float below, float above,
+                                              bool first_lane) {
+  if (first_lane) {  // the slots of the two ends are used for nothing else
     acc[padded(0)] = below;
-    acc[padded(last)] += above;  // reach 0: both ends are one slot
+    acc[padded(p.last)] = above;
   }
   __syncthreads();
-  float* out = p.partial + ((long long)h * p.blocks_per_head + part) * (last + 1);
-  for (int x = threadIdx.x; x <= last; x += blockDim.x) {
+  float* out = p.partial + ((long long)h * p.blocks_per_head + part) * (p.last + 1);
+  for (int x = threadIdx.x; x <= p.last; x += blockDim.x) {
     float t = 0.f;
     for (int q = 0; q < groups; ++q) t += all[q * words + padded(x)];
     out[x] = t;
   }
 }
 
-// A row to a whole block, any length: two passes over the row, of which the second finds it in the caches.
+// Sum over a block for a last step, with two barriers.
 __device__ __forceinline__ float block_sum(float v, float* sh) {
   v = group_sum(v, 32);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
@@ -333,6 +364,89 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
   __syncthreads();
   return v;
 }
+
+template <typename T, int VEC, int NV, int WARPS, bool MASKED, bool EDGE>
+__global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS, 768)) bias_softmax_bwd_rows(const __grid_constant__ Args p) {
+  extern __shared__ float lut[];
+  __shared__ float meet[2][WARPS];
+  __shared__ float red[32];
+  const int words = padded(p.last) + 1;
+  const int h = blockIdx.x / p.blocks_per_head, part = blockIdx.x % p.blocks_per_head;
+  const int G = WARPS == 1 ? p.group : 32, lanes = G * WARPS;
+  const int gl = WARPS == 1 ? threadIdx.x & (G - 1) : threadIdx.x, groups = WARPS == 1 ? blockDim.x / G : 1;
+  float* all = lut + words;
+  float* acc = all + (WARPS == 1 ? (threadIdx.x / G) * words : 0);
+  fill_lut(lut, p, h);
+  if (p.partial)
+    for (int x = threadIdx.x; x < groups * words; x += blockDim.x) all[x] = 0.f;
+  __syncthreads();
+  float below = 0.f, above = 0.f;
+  const unsigned r0 = part * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
+  const unsigned r = WARPS == 1 ? r0 + threadIdx.x / G : r0;
+  RowWalk walk(p, min(r, p.rows - 1), h);
+  int turn = 0;
+  for (unsigned done = 0; r0 + done < r1; done += groups, turn ^= 1) {
+    const bool live = r + done < r1;
+    const T* s = static_cast<const T*>(p.s) + walk.at;
+    const T* g = static_cast<const T*>(p.g) + walk.at;
+    const int phase = EDGE ? (int)((reinterpret_cast<uintptr_t>(s) / sizeof(T)) & (VEC - 1)) : 0;
+    const MaskRow mask = MASKED ? mask_row<VEC>(p, walk.mask, phase) : MaskRow{};
+    const int first_x = walk.first_x(p);
+    const float2 st = p.stats[walk.stat];
+    Pack<T, VEC> raw[NV], graw[NV];  // the gradient waits in its own type: half the registers for 16 bits
+    float2 a[NV][VEC / 2], dot2 = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int j0 = (gl + n * lanes) * VEC - phase;
+      if (j0 < p.Lk) {
+        raw[n] = load_part<T, VEC, EDGE>(s, j0, p.Lk);
+        graw[n] = load_part<T, VEC, EDGE>(g, j0, p.Lk);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int j0 = (gl + n * lanes) * VEC - phase;
+      if (j0 < p.Lk) {
+        to_logits<T, VEC, MASKED, EDGE>(p, lut, mask, j0, first_x + j0, raw[n], a[n]);
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k) {
+          a[n][k] = mul2(weights_of(a[n][k], both(-st.x)), both(st.y));
+          float2 g2 = pair_of(graw[n], k);
+          if (MASKED) g2 = make_float2(a[n][k].x == 0.f ? 0.f : g2.x, a[n][k].y == 0.f ? 0.f : g2.y);  // an excluded key counts nothing
+          dot2 = fma2(a[n][k], g2, dot2);
+        }
+      }
+    }
+    // (with its barrier this row's sums over distances come behind the last row's)
+    const float2 dot = both(-join_sums<WARPS>(group_sum(dot2.x + dot2.y, G), meet, turn));
+    if (live) {
+      T* o = static_cast<T*>(p.out) + walk.at;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int j0 = (gl + n * lanes) * VEC - phase;
+        if (j0 < p.Lk) {
+#pragma unroll
+          for (int k = 0; k < VEC / 2; ++k) {
+            float2 d = mul2(a[n][k], add2(pair_of(graw[n], k), dot));
+            if (MASKED) d = make_float2(a[n][k].x == 0.f ? 0.f : d.x, a[n][k].y == 0.f ? 0.f : d.y);
+            a[n][k] = d;
+            set_pair(raw[n], k, mul2(d, both(p.scale)));
+          }
+          store_part<T, VEC, EDGE>(o, j0, p.Lk, raw[n]);
+          if (p.partial) add_distances<VEC>(acc, p.last, first_x + j0, a[n], below, above);
+        }
+      }
+      if (r + done + groups < r1) walk.advance(p, groups);
+    }
+    if (WARPS == 1) __syncwarp();  // the next row of this group adds to the same sums from other lanes
+  }
+  if (!p.partial) return;
+  below = WARPS == 1 ? group_sum(below, G) : block_sum(below, red);
+  above = WARPS == 1 ? group_sum(above, G) : block_sum(above, red);
+  write_partial(p, all, groups, words, acc, h, part, below, above, gl == 0);
+}
+
+// A row to a whole block, any length: two passes over the row, of which the second finds it in the caches.
 __device__ __forceinline__ float block_max(float v, float* sh) {
   v = group_max(v, 32);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
@@ -342,7 +456,7 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
   return v;
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool MASKED>
 __global__ void __launch_bounds__(kMaxThreads) bias_softmax_fwd_long(const __grid_constant__ Args p) {
   extern __shared__ float lut[];
   __shared__ float sh[32];
@@ -350,45 +464,46 @@ __global__ void __launch_bounds__(kMaxThreads) bias_softmax_fwd_long(const __gri
   fill_lut(lut, p, h);
   __syncthreads();
   const unsigned r0 = part * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
-  for (unsigned r = r0; r < r1; ++r) {
-    const RowAt w = row_at(p, r, h);
-    const T* s = static_cast<const T*>(p.s) + w.at;
+  RowWalk walk(p, r0, h);
+  for (unsigned r = r0; r < r1; ++r, walk.advance(p, 1)) {
+    const T* s = static_cast<const T*>(p.s) + walk.at;
     const int phase = (int)((reinterpret_cast<uintptr_t>(s) / sizeof(T)) & (VEC - 1));
+    const MaskRow mask = MASKED ? mask_row<VEC>(p, walk.mask, phase) : MaskRow{};
+    const int first_x = walk.first_x(p);
     float m = kNegInf, sum = 0.f;
     for (int j0 = (int)threadIdx.x * VEC - phase; j0 < p.Lk; j0 += blockDim.x * VEC) {
-      float a[VEC], top = kNegInf;
-      load_part<T, VEC>(s, j0, p.Lk, a);
-      to_logits<VEC>(p, lut, w.mask_row, j0, w.first_x + j0, a);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) top = fmaxf(top, a[k]);
+      float2 a[VEC / 2], sum2 = make_float2(0.f, 0.f);
+      to_logits<T, VEC, MASKED, true>(p, lut, mask, j0, first_x + j0, load_part<T, VEC, true>(s, j0, p.Lk), a);
+      const float top = max_of(kNegInf, a);
       if (top > m) {
-        sum *= __expf(m - top);  // m = -inf: 0
+        sum *= weight_of(m, top);  // m = -inf: 0
         m = top;
       }
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) sum += weight_of(a[k], m);
+      for (int k = 0; k < VEC / 2; ++k) sum2 = add2(sum2, weights_of(a[k], both(-finite_max(m))));
+      sum += sum2.x + sum2.y;
     }
-    const float all = block_max(m, sh);
-    sum = block_sum(m == kNegInf ? sum : sum * __expf(m - all), sh);  // m = -inf: 0, or NaN from a NaN score
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T* o = static_cast<T*>(p.out) + w.at;
+    const float all = finite_max(block_max(m, sh));
+    sum = block_sum(sum * weight_of(m, all), sh);
+    const float inv = inverse_sum(sum);
+    T* o = static_cast<T*>(p.out) + walk.at;
     for (int j0 = (int)threadIdx.x * VEC - phase; j0 < p.Lk; j0 += blockDim.x * VEC) {
-      float a[VEC];
-      load_part<T, VEC>(s, j0, p.Lk, a);
-      to_logits<VEC>(p, lut, w.mask_row, j0, w.first_x + j0, a);
+      float2 a[VEC / 2];
+      Pack<T, VEC> raw = load_part<T, VEC, true>(s, j0, p.Lk);
+      to_logits<T, VEC, MASKED, true>(p, lut, mask, j0, first_x + j0, raw, a);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) a[k] = weight_of(a[k], all) * inv;
-      store_part<T, VEC>(o, j0, p.Lk, a);
+      for (int k = 0; k < VEC / 2; ++k) set_pair(raw, k, mul2(weights_of(a[k], both(-all)), both(inv)));
+      store_part<T, VEC, true>(o, j0, p.Lk, raw);
     }
-    if (p.stats && threadIdx.x == 0) p.stats[w.stat] = make_float2(all, inv);
+    if (p.stats && threadIdx.x == 0) p.stats[walk.stat] = make_float2(all, inv);
   }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool MASKED>
 __global__ void __launch_bounds__(kMaxThreads) bias_softmax_bwd_long(const __grid_constant__ Args p) {
   extern __shared__ float lut[];
   __shared__ float sh[32];
-  const int last = 2 * p.reach, words = padded(last) + 1;
+  const int words = padded(p.last) + 1;
   const int h = blockIdx.x / p.blocks_per_head, part = blockIdx.x % p.blocks_per_head;
   float* acc = lut + words;
   fill_lut(lut, p, h);
@@ -397,67 +512,59 @@ __global__ void __launch_bounds__(kMaxThreads) bias_softmax_bwd_long(const __gri
   __syncthreads();
   float below = 0.f, above = 0.f;
   const unsigned r0 = part * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
-  for (unsigned r = r0; r < r1; ++r) {
-    const RowAt w = row_at(p, r, h);
-    const T* s = static_cast<const T*>(p.s) + w.at;
-    const T* g = static_cast<const T*>(p.g) + w.at;
+  RowWalk walk(p, r0, h);
+  for (unsigned r = r0; r < r1; ++r, walk.advance(p, 1)) {
+    const T* s = static_cast<const T*>(p.s) + walk.at;
+    const T* g = static_cast<const T*>(p.g) + walk.at;
     const int phase = (int)((reinterpret_cast<uintptr_t>(s) / sizeof(T)) & (VEC - 1));
-    const float2 st = p.stats[w.stat];
+    const MaskRow mask = MASKED ? mask_row<VEC>(p, walk.mask, phase) : MaskRow{};
+    const int first_x = walk.first_x(p);
+    const float2 st = p.stats[walk.stat];
     float dot = 0.f;
-    for (int j0 = (int)threadIdx.x * VEC - phase; j0 < p.Lk; j0 += blockDim.x * VEC) {
-      float a[VEC], d[VEC];
-      load_part<T, VEC>(s, j0, p.Lk, a);
-      load_part<T, VEC>(g, j0, p.Lk, d);
-      to_logits<VEC>(p, lut, w.mask_row, j0, w.first_x + j0, a);
+    for (int pass = 0; pass < 2; ++pass) {
+      T* o = static_cast<T*>(p.out) + walk.at;
+      float2 dot2 = make_float2(0.f, 0.f);
+      for (int j0 = (int)threadIdx.x * VEC - phase; j0 < p.Lk; j0 += blockDim.x * VEC) {
+        float2 a[VEC / 2];
+        Pack<T, VEC> raw = load_part<T, VEC, true>(s, j0, p.Lk);
+        const Pack<T, VEC> graw = load_part<T, VEC, true>(g, j0, p.Lk);
+        to_logits<T, VEC, MASKED, true>(p, lut, mask, j0, first_x + j0, raw, a);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const float q = weight_of(a[k], st.x) * st.y;
-        dot += q == 0.f ? 0.f : q * d[k];
+        for (int k = 0; k < VEC / 2; ++k) {
+          const float2 q = mul2(weights_of(a[k], both(-st.x)), both(st.y));
+          float2 d = mul2(q, add2(pair_of(graw, k), both(-dot)));  // first pass: dot = 0
+          if (MASKED) d = make_float2(q.x == 0.f ? 0.f : d.x, q.y == 0.f ? 0.f : d.y);
+          dot2 = add2(dot2, d);
+          a[k] = d;
+          set_pair(raw, k, mul2(d, both(p.scale)));
+        }
+        if (pass) {
+          store_part<T, VEC, true>(o, j0, p.Lk, raw);
+          if (p.partial) add_distances<VEC>(acc, p.last, first_x + j0, a, below, above);
+        }
       }
-    }
-    dot = block_sum(dot, sh);  // its barriers also order this row's sums over distances behind the last row's
-    T* o = static_cast<T*>(p.out) + w.at;
-    for (int j0 = (int)threadIdx.x * VEC - phase; j0 < p.Lk; j0 += blockDim.x * VEC) {
-      float a[VEC], d[VEC];
-      load_part<T, VEC>(s, j0, p.Lk, a);
-      load_part<T, VEC>(g, j0, p.Lk, d);
-      to_logits<VEC>(p, lut, w.mask_row, j0, w.first_x + j0, a);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const float q = weight_of(a[k], st.x) * st.y;
-        d[k] = q == 0.f ? 0.f : q * (d[k] - dot);
-        a[k] = d[k] * p.scale;
-      }
-      store_part<T, VEC>(o, j0, p.Lk, a);
-      if (p.partial) add_distances<VEC>(acc, last, w.first_x + j0, d, below, above);
+      if (!pass) dot = block_sum(dot2.x + dot2.y, sh);  // its barriers also order this row's sums over distances behind the last row's
     }
   }
   if (!p.partial) return;
   below = block_sum(below, sh);
   above = block_sum(above, sh);
-  if (threadIdx.x == 0) {
-    acc[padded(0)] = below;
-    acc[padded(last)] += above;
-  }
-  __syncthreads();
-  float* out = p.partial + ((long long)h * p.blocks_per_head + part) * (last + 1);
-  for (int x = threadIdx.x; x <= last; x += blockDim.x) out[x] = acc[padded(x)];
+  write_partial(p, acc, 1, words, acc, h, part, below, above, threadIdx.x == 0);
 }
 
 // One block per head and bucket: sums over the blocks' partial sums for the distances of the bucket, in a fixed order.  A
 // bucket's distances are neighbours, so its slots are one run [x0, x1].
-__global__ void __launch_bounds__(kMaxThreads) bias_table_grad(const float* partial, int blocks, int reach, const __grid_constant__ B200RelativeBuckets rb,
+__global__ void __launch_bounds__(kMaxThreads) bias_table_grad(const float* partial, int blocks, int reach, int last, const __grid_constant__ B200RelativeBuckets rb,
                                                                int H, void* out, int dtype) {
   __shared__ float sh[32];
-  const int h = blockIdx.x, bucket = blockIdx.y, slots = 2 * reach + 1;
+  const int h = blockIdx.x, bucket = blockIdx.y, slots = last + 1;
   const bool upper = rb.bidirectional && bucket >= rb.per_side;
   const int c = upper ? bucket - rb.per_side : bucket, far = c - rb.exact;
   int lo = far >= 0 ? rb.first[far] : c;
   int hi = c == rb.per_side - 1 ? reach : (far >= 0 ? rb.first[far + 1] : c + 1) - 1;
   if (upper && lo == 0) lo = 1;  // distance 0 belongs to the lower half
   hi = min(hi, reach);
-  int x0 = upper ? reach + lo : reach - hi, x1 = upper ? reach + hi : reach - lo;
-  if (!rb.bidirectional && c == 0) x1 = 2 * reach;  // keys after the query
+  const int x0 = upper ? reach + lo : reach - hi, x1 = upper ? reach + hi : reach - lo;
   float t = 0.f;
   if (lo <= hi) {
     const float* mine = partial + (long long)h * blocks * slots + x0;
@@ -475,7 +582,8 @@ __global__ void __launch_bounds__(kMaxThreads) bias_table_grad(const float* part
 
 struct Plan {
   Args a;
-  int threads, nv;  // nv 0: a block per row
+  int threads, nv, warps;  // nv 0: any length
+  bool edge;
   size_t smem;
 };
 
@@ -488,21 +596,26 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
   a.mk_b = p.mask_stride[0]; a.mk_h = p.mask_stride[1]; a.mk_i = p.mask_stride[2]; a.mk_j = p.mask_stride[3];
   a.H = p.H; a.Lq = p.Lq; a.Lk = p.Lk; a.offset = p.query_offset; a.scale = p.scale; a.rb = p.buckets;
   a.rows = (unsigned)((long long)p.B * p.Lq);
-  // beyond the farthest distance of this call nothing has to be told apart either
+  // beyond the farthest distance of this call nothing has to be told apart either, nor after the query if those keys
+  // share a bucket
   const long long ahead = (long long)p.Lk - 1 - p.query_offset, behind = (long long)p.Lq - 1 + p.query_offset;
   long long far = ahead > behind ? ahead : behind;
   if (far < -ahead) far = -ahead;
   if (far < -behind) far = -behind;
   a.reach = (int)(far + 1 < p.buckets.max_distance ? far + 1 : p.buckets.max_distance);
+  a.last = p.buckets.bidirectional ? 2 * a.reach : a.reach;
   const int vec = p.dtype == B200_F32 ? 4 : 8;
   const bool aligned = p.Lk % vec == 0 && p.stride[0] % vec == 0 && p.stride[1] % vec == 0 && p.stride[2] % vec == 0;
   const int nvec = aligned ? p.Lk / vec : (p.Lk + 2 * vec - 2) / vec;  // an unaligned row may touch one vector more
-  const int words = 2 * a.reach + (2 * a.reach >> 5) + 1;
+  const int words = padded(a.last) + 1;
+  pl.edge = !aligned;
   pl.threads = kMaxThreads;
-  int groups;
-  if (nvec <= 32 * 4) {
+  pl.warps = 1;
+  int groups = 1;
+  const int wide = 16 / vec;  // vectors for 16 elements in a lane
+  if (nvec <= 32 * wide) {
     int G = 1;
-    while (G < nvec && G < 32) G <<= 1;
+    while (G * wide < nvec) G <<= 1;
     if (bwd)  // sums over distances for each group: wider groups where there would be too many
       while (G < 32 && (kMaxThreads / G) * words * 4 > 64 * 1024) G <<= 1;
     a.group = G;
@@ -511,11 +624,13 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
     if (bwd)
       while (pl.threads > 32 && (pl.threads / G + 1) * words * 4 > 96 * 1024) pl.threads >>= 1;
     groups = pl.threads / G;
-    pl.smem = (size_t)(bwd ? groups + 1 : 1) * words * 4;
-  } else {
-    groups = 1;
-    pl.smem = (size_t)(bwd ? 2 : 1) * words * 4;
+  } else if (nvec <= kMaxThreads * 4) {
+    pl.nv = nvec <= kMaxThreads * wide ? wide : 4;
+    pl.warps = 2;
+    while (pl.warps * 32 * pl.nv < nvec) pl.warps *= 2;
+    pl.threads = 32 * pl.warps;
   }
+  pl.smem = (size_t)(bwd ? groups + 1 : 1) * words * 4;
   long long blocks = 148LL * 8 * kMaxThreads / pl.threads / (p.H > 0 ? p.H : 1);
   const long long most = ((long long)a.rows + groups - 1) / groups;
   if (blocks > most) blocks = most;
@@ -529,7 +644,7 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
 
 template <typename K>
 int launch(K kernel, const Plan& pl, cudaStream_t s) {
-  if (pl.smem > 48 * 1024) {
+  if (pl.smem > 48 * 1024 - 512) {  // beside the static part
     const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem);
     if (e != cudaSuccess) return (int)e;
   }
@@ -537,19 +652,32 @@ int launch(K kernel, const Plan& pl, cudaStream_t s) {
   return (int)cudaGetLastError();
 }
 
-template <typename T, int VEC>
-int dispatch(const Plan& pl, bool bwd, cudaStream_t s) {
-  switch (pl.nv) {
-    case 1: return bwd ? launch(bias_softmax_bwd_rows<T, VEC, 1>, pl, s) : launch(bias_softmax_fwd_rows<T, VEC, 1>, pl, s);
-    case 2: return bwd ? launch(bias_softmax_bwd_rows<T, VEC, 2>, pl, s) : launch(bias_softmax_fwd_rows<T, VEC, 2>, pl, s);
-    case 4: return bwd ? launch(bias_softmax_bwd_rows<T, VEC, 4>, pl, s) : launch(bias_softmax_fwd_rows<T, VEC, 4>, pl, s);
-    default: return bwd ? launch(bias_softmax_bwd_long<T, VEC>, pl, s) : launch(bias_softmax_fwd_long<T, VEC>, pl, s);
-  }
+template <typename T, int VEC, int NV, int WARPS, bool BWD, bool MASKED>
+int launch_rows(const Plan& pl, cudaStream_t s) {
+  if (pl.edge)
+    return BWD ? launch(bias_softmax_bwd_rows<T, VEC, NV, WARPS, MASKED, true>, pl, s) : launch(bias_softmax_fwd_rows<T, VEC, NV, WARPS, MASKED, true>, pl, s);
+  return BWD ? launch(bias_softmax_bwd_rows<T, VEC, NV, WARPS, MASKED, false>, pl, s) : launch(bias_softmax_fwd_rows<T, VEC, NV, WARPS, MASKED, false>, pl, s);
 }
-int dispatch_type(const Plan& pl, int dtype, bool bwd, cudaStream_t s) {
-  if (dtype == B200_BF16) return dispatch<__nv_bfloat16, 8>(pl, bwd, s);
-  if (dtype == B200_F16) return dispatch<__half, 8>(pl, bwd, s);
-  if (dtype == B200_F32) return dispatch<float, 4>(pl, bwd, s);
+template <typename T, int VEC, bool BWD, bool MASKED>
+int dispatch(const Plan& pl, cudaStream_t s) {
+  constexpr int kWide = 16 / VEC;
+  if (pl.nv == 0) return BWD ? launch(bias_softmax_bwd_long<T, VEC, MASKED>, pl, s) : launch(bias_softmax_fwd_long<T, VEC, MASKED>, pl, s);
+  if (pl.warps == 1) {
+    if (pl.nv == 1) return launch_rows<T, VEC, 1, 1, BWD, MASKED>(pl, s);
+    if (pl.nv == 2) return launch_rows<T, VEC, 2, 1, BWD, MASKED>(pl, s);
+    return launch_rows<T, VEC, kWide, 1, BWD, MASKED>(pl, s);  // kWide = 2: not reached
+  }
+  if (pl.nv != kWide) return launch_rows<T, VEC, 4, 8, BWD, MASKED>(pl, s);
+  if (pl.warps == 2) return launch_rows<T, VEC, kWide, 2, BWD, MASKED>(pl, s);
+  if (pl.warps == 4) return launch_rows<T, VEC, kWide, 4, BWD, MASKED>(pl, s);
+  return launch_rows<T, VEC, kWide, 8, BWD, MASKED>(pl, s);
+}
+template <bool BWD>
+int dispatch_type(const Plan& pl, int dtype, cudaStream_t s) {
+  const bool masked = pl.a.mask != nullptr;
+  if (dtype == B200_BF16) return masked ? dispatch<__nv_bfloat16, 8, BWD, true>(pl, s) : dispatch<__nv_bfloat16, 8, BWD, false>(pl, s);
+  if (dtype == B200_F16) return masked ? dispatch<__half, 8, BWD, true>(pl, s) : dispatch<__half, 8, BWD, false>(pl, s);
+  if (dtype == B200_F32) return masked ? dispatch<float, 4, BWD, true>(pl, s) : dispatch<float, 4, BWD, false>(pl, s);
   return (int)cudaErrorInvalidValue;
 }
 
@@ -566,13 +694,13 @@ bool empty(const B200BiasSoftmax* p) { return (long long)p->B * p->Lq == 0 || p-
 extern "C" int b200_bias_softmax_fwd(const B200BiasSoftmax* p, void* stream) {
   if (!valid(p)) return (int)cudaErrorInvalidValue;
   if (empty(p)) return 0;
-  return dispatch_type(make_plan(*p, false), p->dtype, false, (cudaStream_t)stream);
+  return dispatch_type<false>(make_plan(*p, false), p->dtype, (cudaStream_t)stream);
 }
 
 extern "C" long long b200_bias_softmax_workspace(const B200BiasSoftmax* p) {
   if (!valid(p) || empty(p) || !p->dtable) return 0;
   const Plan pl = make_plan(*p, true);
-  return (long long)p->H * pl.a.blocks_per_head * (2 * pl.a.reach + 1) * (long long)sizeof(float);
+  return (long long)p->H * pl.a.blocks_per_head * (pl.a.last + 1) * (long long)sizeof(float);
 }
 
 extern "C" int b200_bias_softmax_bwd(const B200BiasSoftmax* p, void* workspace, void* stream) {
@@ -585,10 +713,10 @@ extern "C" int b200_bias_softmax_bwd(const B200BiasSoftmax* p, void* workspace, 
   }
   Plan pl = make_plan(*p, true);
   pl.a.partial = p->dtable ? static_cast<float*>(workspace) : nullptr;
-  const int rc = dispatch_type(pl, p->dtype, true, s);
+  const int rc = dispatch_type<true>(pl, p->dtype, s);
   if (rc || !p->dtable) return rc;
   const int buckets = p->buckets.per_side * (p->buckets.bidirectional ? 2 : 1);
-  bias_table_grad<<<dim3((unsigned)p->H, (unsigned)buckets), kMaxThreads, 0, s>>>(pl.a.partial, pl.a.blocks_per_head, pl.a.reach, p->buckets, p->H,
+  bias_table_grad<<<dim3((unsigned)p->H, (unsigned)buckets), kMaxThreads, 0, s>>>(pl.a.partial, pl.a.blocks_per_head, pl.a.reach, pl.a.last, p->buckets, p->H,
                                                                                 p->dtable, p->table_dtype);
   return (int)cudaGetLastError();
 }

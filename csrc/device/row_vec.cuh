@@ -33,6 +33,46 @@ __device__ __forceinline__ void store(T* __restrict__ p, const float (&in)[N]) {
   *reinterpret_cast<Pack<T, N>*>(p) = raw;
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// Neighbouring elements of a pack as fp32, and back.
+template <typename T, int N>
+__device__ __forceinline__ float2 pair_of(const Pack<T, N>& p, int i) { return make_float2(to_f32<T>(p.v[2 * i]), to_f32<T>(p.v[2 * i + 1])); }
+template <int N>
+__device__ __forceinline__ void set_pair(Pack<float, N>& p, int i, float2 v) { p.v[2 * i] = v.x; p.v[2 * i + 1] = v.y; }
+template <int N>
+__device__ __forceinline__ void set_pair(Pack<__nv_bfloat16, N>& p, int i, float2 v) {
+  *reinterpret_cast<__nv_bfloat162*>(&p.v[2 * i]) = __float22bfloat162_rn(v);
+}
+template <int N>
+__device__ __forceinline__ void set_pair(Pack<__half, N>& p, int i, float2 v) { *reinterpret_cast<__half2*>(&p.v[2 * i]) = __float22half2_rn(v); }
+
+// 2^x; results below the smallest normal number become 0
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Sums over aligned groups of `width` lanes (a power of two up to 32); every lane of the warp takes part.
 __device__ __forceinline__ float group_sum(float v, int width) {
   for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

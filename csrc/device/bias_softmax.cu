@@ -13,6 +13,7 @@
 // for every group of lanes that walks over rows of its own.  In one row no two elements have the same distance, so no atomics
 // are needed and the order of every sum is fixed: the same inputs give the same bits.
 #include "kernels_api.h"
+#include <cstdlib>
 #include "row_vec.cuh"
 
 namespace {
@@ -31,6 +32,7 @@ struct Args {
   const void* table;
   const void* mask;     // or null
   long long st_b, st_h, st_i;     // of s, g and out (their last dimension is dense)
+  long long elements;             // of s
   long long mk_b, mk_h, mk_i, mk_j;
   int table_dtype, mask_dtype;
   int H, Lq, Lk, offset;
@@ -64,6 +66,10 @@ __device__ __forceinline__ int bucket_of(int rel, const B200RelativeBuckets& rb)
 // One pad word every 32: lanes that read eight neighbours each then meet in different banks.
 __host__ __device__ __forceinline__ int padded(int x) { return x + (x >> 5); }
 
+// Words of shared memory in front of the rows on their way, which begin on a 16-byte boundary.
+__host__ __device__ __forceinline__ int ring_offset(int last) { return (padded(last) + 1 + 3) & ~3; }
+__host__ __device__ __forceinline__ int ring_offset_bwd(int last, int groups) { return ((groups + 1) * (padded(last) + 1) + 3) & ~3; }
+
 __device__ __forceinline__ void fill_lut(float* lut, const Args& p, int h) {
   for (int x = threadIdx.x; x <= p.last; x += blockDim.x)
     lut[padded(x)] = scalar_at(p.table, (long long)bucket_of(x - p.reach, p.rb) * p.H + h, p.table_dtype);
@@ -71,6 +77,7 @@ __device__ __forceinline__ void fill_lut(float* lut, const Args& p, int h) {
 
 // Vectors of VEC elements (16 bytes) on 16-byte boundaries.  EDGE: rows may begin anywhere and have any length, so that the
 // first and the last vector can reach over the row's ends; without it (rows begin on boundaries and have whole vectors) those tests are gone.
+// FULL: besides, the row fills every vector of its lanes.
 // The elements [j0, j0 + VEC) of a row; those outside [0, n) read as 0 and are not written.
 template <typename T, int VEC, bool EDGE>
 __device__ __forceinline__ Pack<T, VEC> load_part(const T* row, int j0, int n) {
@@ -182,7 +189,7 @@ __device__ __forceinline__ float2 weights_of(float2 a, float2 minus_m) {
 }
 __device__ __forceinline__ float finite_max(float m) { return m == kNegInf ? 0.f : m; }
 // 1 / sum, 0 for a row with nothing left (a NaN stays one)
-__device__ __forceinline__ float inverse_sum(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+__device__ __forceinline__ float inverse_sum(float sum) { return sum == 0.f ? 0.f : __fdividef(1.f, sum); }
 template <int N>
 __device__ __forceinline__ float max_of(float m, const float2 (&a)[N]) {
 #pragma unroll
@@ -255,43 +262,86 @@ __device__ __forceinline__ float2 join_rows(float m, float sum, int G, float2 (*
   return make_float2(top, all);
 }
 
+// Rows on their way: each thread copies its vectors of the next rows to a place of its own in shared memory, so that several
+// kilobytes for every block are under way while a row is worked on, at no registers.  An EDGE vector is copied whole, neighbours' elements
+// and all, as long as it lies in the tensor; the very last one of the tensor may not and is read element by element when its turn comes.
+constexpr int ring_depth(int nv, bool bwd) { return nv == 1 ? 4 : (nv == 2 ? (bwd ? 3 : 4) : 2); }
+template <typename T, int VEC, int NV, bool EDGE, bool FULL>
+struct RowVectors {
+  static __device__ __forceinline__ int phase_of(const T* row) { return EDGE ? (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) & (VEC - 1)) : 0; }
+  // this thread's vectors of a row to slots `blockDim.x` apart
+  static __device__ __forceinline__ void fetch(const T* base, long long elements, long long at, int Lk, int gl, int lanes, Pack<T, VEC>* slot) {
+    const int phase = phase_of(base + at);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int j0 = (gl + n * lanes) * VEC - phase;
+      if ((FULL || j0 < Lk) && (!EDGE || at + j0 + VEC <= elements)) copy16_async(slot + n * blockDim.x, base + at + j0);
+    }
+  }
+  static __device__ __forceinline__ void take(const T* base, long long elements, long long at, int Lk, int gl, int lanes, const Pack<T, VEC>* slot,
+                                              Pack<T, VEC> (&v)[NV]) {
+    const int phase = phase_of(base + at);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int j0 = (gl + n * lanes) * VEC - phase;
+      if (FULL || j0 < Lk) {
+        if (!EDGE || at + j0 + VEC <= elements) v[n] = slot[n * blockDim.x];
+        else v[n] = load_part<T, VEC, true>(base + at, j0, Lk);
+      }
+    }
+  }
+};
+
 // Registers: 64 a thread forward and 80 backward hold 16 elements of a lane and leave 1024 and 768 threads for an SM.  Left alone, the
 // compiler takes 120 for the loads of a mask whose keys are not side by side, which is the rare case.
 constexpr int row_threads(int warps) { return warps == 1 ? kMaxThreads : 32 * warps; }
 constexpr int row_blocks(int elements, int warps, int resident) { return elements <= 16 ? resident / row_threads(warps) : 1; }
 
 // A row in registers: NV vectors of VEC elements for each of its lanes (a group of G of one warp, or the block's WARPS warps).
-template <typename T, int VEC, int NV, int WARPS, bool MASKED, bool EDGE>
+template <typename T, int VEC, int NV, int WARPS, bool MASKED, bool EDGE, bool FULL>
 __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS, 1024)) bias_softmax_fwd_rows(const __grid_constant__ Args p) {
-  extern __shared__ float lut[];
+  extern __shared__ __align__(16) float lut[];
   __shared__ float2 meet[2][WARPS];
   const int h = blockIdx.x / p.blocks_per_head, part = blockIdx.x % p.blocks_per_head;
-  fill_lut(lut, p, h);
-  __syncthreads();
   const int G = WARPS == 1 ? p.group : 32, lanes = G * WARPS;
   const int gl = WARPS == 1 ? threadIdx.x & (G - 1) : threadIdx.x, groups = WARPS == 1 ? blockDim.x / G : 1;
   const unsigned r0 = part * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
   const unsigned r = WARPS == 1 ? r0 + threadIdx.x / G : r0;
-  RowWalk walk(p, min(r, p.rows - 1), h);  // a group behind the last row follows on rows that are there
-  int turn = 0;
+  using Vectors = RowVectors<T, VEC, NV, EDGE, FULL>;
+  constexpr int kDepth = ring_depth(NV, false);
+  const T* base = static_cast<const T*>(p.s);
+  Pack<T, VEC>* ring = reinterpret_cast<Pack<T, VEC>*>(lut + ring_offset(p.last)) + threadIdx.x;
+  RowWalk row(p, min(r, p.rows - 1), h), ahead = row;  // a group behind the last row follows on rows that are there
+  unsigned fetched = 0;
+  auto fetch_next = [&](int stage) {
+    if (r + fetched < r1) {
+      Vectors::fetch(base, p.elements, ahead.at, p.Lk, gl, lanes, ring + stage * NV * blockDim.x);
+      fetched += groups;
+      if (r + fetched < r1) ahead.advance(p, groups);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int d = 0; d < kDepth - 1; ++d) fetch_next(d);
+  fill_lut(lut, p, h);
+  __syncthreads();
+  int turn = 0, stage = 0;
   for (unsigned done = 0; r0 + done < r1; done += groups, turn ^= 1) {
     const bool live = r + done < r1;
-    const T* s = static_cast<const T*>(p.s) + walk.at;
-    const int phase = EDGE ? (int)((reinterpret_cast<uintptr_t>(s) / sizeof(T)) & (VEC - 1)) : 0;
-    const MaskRow mask = MASKED ? mask_row<VEC>(p, walk.mask, phase) : MaskRow{};
-    const int first_x = walk.first_x(p);
+    fetch_next(stage == 0 ? kDepth - 1 : stage - 1);
+    copies_wait<kDepth - 1>();
     Pack<T, VEC> raw[NV];
+    Vectors::take(base, p.elements, row.at, p.Lk, gl, lanes, ring + stage * NV * blockDim.x, raw);
+    stage = stage == kDepth - 1 ? 0 : stage + 1;
+    const int phase = Vectors::phase_of(base + row.at);
+    const MaskRow mask = MASKED ? mask_row<VEC>(p, row.mask, phase) : MaskRow{};
+    const int first_x = row.first_x(p);
     float2 a[NV][VEC / 2];
     float m = kNegInf;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int j0 = (gl + n * lanes) * VEC - phase;
-      if (j0 < p.Lk) raw[n] = load_part<T, VEC, EDGE>(s, j0, p.Lk);
-    }
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int j0 = (gl + n * lanes) * VEC - phase;
-      if (j0 < p.Lk) {
+      if (FULL || j0 < p.Lk) {
         to_logits<T, VEC, MASKED, EDGE>(p, lut, mask, j0, first_x + j0, raw[n], a[n]);
         m = max_of(m, a[n]);
       }
@@ -301,7 +351,7 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
     float2 sum2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      if ((gl + n * lanes) * VEC - phase < p.Lk) {
+      if (FULL || (gl + n * lanes) * VEC - phase < p.Lk) {
 #pragma unroll
         for (int k = 0; k < VEC / 2; ++k) {
           a[n][k] = weights_of(a[n][k], minus);
@@ -309,21 +359,21 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
         }
       }
     }
-    const float2 row = join_rows<WARPS>(m, group_sum(sum2.x + sum2.y, G), G, meet, turn);
-    const float inv = inverse_sum(row.y), f = WARPS == 1 ? inv : inv * weight_of(m, finite_max(row.x));
+    const float2 all = join_rows<WARPS>(m, group_sum(sum2.x + sum2.y, G), G, meet, turn);
+    const float inv = inverse_sum(all.y), f = WARPS == 1 ? inv : inv * weight_of(m, finite_max(all.x));
     if (live) {
-      T* o = static_cast<T*>(p.out) + walk.at;
+      T* o = static_cast<T*>(p.out) + row.at;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         const int j0 = (gl + n * lanes) * VEC - phase;
-        if (j0 < p.Lk) {
+        if (FULL || j0 < p.Lk) {
 #pragma unroll
           for (int k = 0; k < VEC / 2; ++k) set_pair(raw[n], k, mul2(a[n][k], both(f)));
           store_part<T, VEC, EDGE>(o, j0, p.Lk, raw[n]);
         }
       }
-      if (p.stats && gl == 0) p.stats[walk.stat] = make_float2(finite_max(row.x), inv);
-      if (r + done + groups < r1) walk.advance(p, groups);
+      if (p.stats && gl == 0) p.stats[row.stat] = make_float2(finite_max(all.x), inv);
+      if (r + done + groups < r1) row.advance(p, groups);
     }
   }
 }
@@ -365,9 +415,9 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
   return v;
 }
 
-template <typename T, int VEC, int NV, int WARPS, bool MASKED, bool EDGE>
+template <typename T, int VEC, int NV, int WARPS, bool MASKED, bool EDGE, bool FULL>
 __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS, 768)) bias_softmax_bwd_rows(const __grid_constant__ Args p) {
-  extern __shared__ float lut[];
+  extern __shared__ __align__(16) float lut[];
   __shared__ float meet[2][WARPS];
   __shared__ float red[32];
   const int words = padded(p.last) + 1;
@@ -376,43 +426,61 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
   const int gl = WARPS == 1 ? threadIdx.x & (G - 1) : threadIdx.x, groups = WARPS == 1 ? blockDim.x / G : 1;
   float* all = lut + words;
   float* acc = all + (WARPS == 1 ? (threadIdx.x / G) * words : 0);
+  float below = 0.f, above = 0.f;
+  const unsigned r0 = part * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
+  const unsigned r = WARPS == 1 ? r0 + threadIdx.x / G : r0;
+  using Vectors = RowVectors<T, VEC, NV, EDGE, FULL>;
+  constexpr int kDepth = ring_depth(NV, true);
+  const T* base = static_cast<const T*>(p.s);
+  const T* gbase = static_cast<const T*>(p.g);
+  Pack<T, VEC>* ring = reinterpret_cast<Pack<T, VEC>*>(lut + ring_offset_bwd(p.last, groups)) + threadIdx.x;
+  RowWalk row(p, min(r, p.rows - 1), h), ahead = row;
+  unsigned fetched = 0;
+  auto fetch_next = [&](int stage) {
+    if (r + fetched < r1) {
+      Vectors::fetch(base, p.elements, ahead.at, p.Lk, gl, lanes, ring + stage * 2 * NV * blockDim.x);
+      Vectors::fetch(gbase, p.elements, ahead.at, p.Lk, gl, lanes, ring + (stage * 2 + 1) * NV * blockDim.x);
+      fetched += groups;
+      if (r + fetched < r1) ahead.advance(p, groups);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int d = 0; d < kDepth - 1; ++d) fetch_next(d);
+  float2 st_next = p.stats[row.stat];
   fill_lut(lut, p, h);
   if (p.partial)
     for (int x = threadIdx.x; x < groups * words; x += blockDim.x) all[x] = 0.f;
   __syncthreads();
-  float below = 0.f, above = 0.f;
-  const unsigned r0 = part * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
-  const unsigned r = WARPS == 1 ? r0 + threadIdx.x / G : r0;
-  RowWalk walk(p, min(r, p.rows - 1), h);
-  int turn = 0;
+  int turn = 0, stage = 0;
   for (unsigned done = 0; r0 + done < r1; done += groups, turn ^= 1) {
     const bool live = r + done < r1;
-    const T* s = static_cast<const T*>(p.s) + walk.at;
-    const T* g = static_cast<const T*>(p.g) + walk.at;
-    const int phase = EDGE ? (int)((reinterpret_cast<uintptr_t>(s) / sizeof(T)) & (VEC - 1)) : 0;
-    const MaskRow mask = MASKED ? mask_row<VEC>(p, walk.mask, phase) : MaskRow{};
-    const int first_x = walk.first_x(p);
-    const float2 st = p.stats[walk.stat];
+    const RowWalk now = row;
+    const float2 st = st_next;
+    if (r + done + groups < r1) {
+      row.advance(p, groups);
+      st_next = p.stats[row.stat];
+    }
+    fetch_next(stage == 0 ? kDepth - 1 : stage - 1);
+    copies_wait<kDepth - 1>();
     Pack<T, VEC> raw[NV], graw[NV];  // the gradient waits in its own type: half the registers for 16 bits
+    Vectors::take(base, p.elements, now.at, p.Lk, gl, lanes, ring + stage * 2 * NV * blockDim.x, raw);
+    Vectors::take(gbase, p.elements, now.at, p.Lk, gl, lanes, ring + (stage * 2 + 1) * NV * blockDim.x, graw);
+    stage = stage == kDepth - 1 ? 0 : stage + 1;
+    const int phase = Vectors::phase_of(base + now.at);
+    const MaskRow mask = MASKED ? mask_row<VEC>(p, now.mask, phase) : MaskRow{};
+    const int first_x = now.first_x(p);
     float2 a[NV][VEC / 2], dot2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int j0 = (gl + n * lanes) * VEC - phase;
-      if (j0 < p.Lk) {
-        raw[n] = load_part<T, VEC, EDGE>(s, j0, p.Lk);
-        graw[n] = load_part<T, VEC, EDGE>(g, j0, p.Lk);
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int j0 = (gl + n * lanes) * VEC - phase;
-      if (j0 < p.Lk) {
+      if (FULL || j0 < p.Lk) {
         to_logits<T, VEC, MASKED, EDGE>(p, lut, mask, j0, first_x + j0, raw[n], a[n]);
 #pragma unroll
         for (int k = 0; k < VEC / 2; ++k) {
           a[n][k] = mul2(weights_of(a[n][k], both(-st.x)), both(st.y));
           float2 g2 = pair_of(graw[n], k);
-          if (MASKED) g2 = make_float2(a[n][k].x == 0.f ? 0.f : g2.x, a[n][k].y == 0.f ? 0.f : g2.y);  // an excluded key counts nothing
+          if (MASKED || EDGE) g2 = make_float2(a[n][k].x == 0.f ? 0.f : g2.x, a[n][k].y == 0.f ? 0.f : g2.y);  // an excluded key counts nothing
           dot2 = fma2(a[n][k], g2, dot2);
         }
       }
@@ -420,15 +488,15 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
     // (with its barrier this row's sums over distances come behind the last row's)
     const float2 dot = both(-join_sums<WARPS>(group_sum(dot2.x + dot2.y, G), meet, turn));
     if (live) {
-      T* o = static_cast<T*>(p.out) + walk.at;
+      T* o = static_cast<T*>(p.out) + now.at;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         const int j0 = (gl + n * lanes) * VEC - phase;
-        if (j0 < p.Lk) {
+        if (FULL || j0 < p.Lk) {
 #pragma unroll
           for (int k = 0; k < VEC / 2; ++k) {
             float2 d = mul2(a[n][k], add2(pair_of(graw[n], k), dot));
-            if (MASKED) d = make_float2(a[n][k].x == 0.f ? 0.f : d.x, a[n][k].y == 0.f ? 0.f : d.y);
+            if (MASKED || EDGE) d = make_float2(a[n][k].x == 0.f ? 0.f : d.x, a[n][k].y == 0.f ? 0.f : d.y);
             a[n][k] = d;
             set_pair(raw[n], k, mul2(d, both(p.scale)));
           }
@@ -436,7 +504,6 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
           if (p.partial) add_distances<VEC>(acc, p.last, first_x + j0, a[n], below, above);
         }
       }
-      if (r + done + groups < r1) walk.advance(p, groups);
     }
     if (WARPS == 1) __syncwarp();  // the next row of this group adds to the same sums from other lanes
   }
@@ -458,7 +525,7 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
 
 template <typename T, int VEC, bool MASKED>
 __global__ void __launch_bounds__(kMaxThreads) bias_softmax_fwd_long(const __grid_constant__ Args p) {
-  extern __shared__ float lut[];
+  extern __shared__ __align__(16) float lut[];
   __shared__ float sh[32];
   const int h = blockIdx.x / p.blocks_per_head, part = blockIdx.x % p.blocks_per_head;
   fill_lut(lut, p, h);
@@ -501,7 +568,7 @@ __global__ void __launch_bounds__(kMaxThreads) bias_softmax_fwd_long(const __gri
 
 template <typename T, int VEC, bool MASKED>
 __global__ void __launch_bounds__(kMaxThreads) bias_softmax_bwd_long(const __grid_constant__ Args p) {
-  extern __shared__ float lut[];
+  extern __shared__ __align__(16) float lut[];
   __shared__ float sh[32];
   const int words = padded(p.last) + 1;
   const int h = blockIdx.x / p.blocks_per_head, part = blockIdx.x % p.blocks_per_head;
@@ -583,7 +650,7 @@ __global__ void __launch_bounds__(kMaxThreads) bias_table_grad(const float* part
 struct Plan {
   Args a;
   int threads, nv, warps;  // nv 0: any length
-  bool edge;
+  bool edge, full;
   size_t smem;
 };
 
@@ -596,6 +663,7 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
   a.mk_b = p.mask_stride[0]; a.mk_h = p.mask_stride[1]; a.mk_i = p.mask_stride[2]; a.mk_j = p.mask_stride[3];
   a.H = p.H; a.Lq = p.Lq; a.Lk = p.Lk; a.offset = p.query_offset; a.scale = p.scale; a.rb = p.buckets;
   a.rows = (unsigned)((long long)p.B * p.Lq);
+  a.elements = (long long)p.B * p.H * p.Lq * p.Lk;
   // beyond the farthest distance of this call nothing has to be told apart either, nor after the query if those keys
   // share a bucket
   const long long ahead = (long long)p.Lk - 1 - p.query_offset, behind = (long long)p.Lq - 1 + p.query_offset;
@@ -630,8 +698,16 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
     while (pl.warps * 32 * pl.nv < nvec) pl.warps *= 2;
     pl.threads = 32 * pl.warps;
   }
+  pl.full = aligned && nvec == pl.nv * (pl.warps == 1 ? a.group : pl.threads);
   pl.smem = (size_t)(bwd ? groups + 1 : 1) * words * 4;
-  long long blocks = 148LL * 8 * kMaxThreads / pl.threads / (p.H > 0 ? p.H : 1);
+  if (pl.nv)
+    pl.smem = (bwd ? ring_offset_bwd(a.last, groups) : ring_offset(a.last)) * 4 + (size_t)ring_depth(pl.nv, bwd) * pl.nv * pl.threads * 16 * (bwd ? 2 : 1);
+  // One wave of blocks: each has to build its table of biases first, and what it leaves for the table gradient has to be added up.
+  int resident = (bwd ? 768 : 1024) / pl.threads;
+  const int by_smem = (int)(220 * 1024 / (pl.smem + 1536));
+  if (resident > by_smem) resident = by_smem > 0 ? by_smem : 1;
+  static const int mult = getenv("CB_M") ? atoi(getenv("CB_M")) : 1;
+  long long blocks = 148LL * resident * mult / (p.H > 0 ? p.H : 1);
   const long long most = ((long long)a.rows + groups - 1) / groups;
   if (blocks > most) blocks = most;
   if (blocks < 1) blocks = 1;
@@ -652,11 +728,16 @@ int launch(K kernel, const Plan& pl, cudaStream_t s) {
   return (int)cudaGetLastError();
 }
 
+template <typename T, int VEC, int NV, int WARPS, bool MASKED, bool EDGE, bool FULL, bool BWD>
+int launch_row(const Plan& pl, cudaStream_t s) {
+  return BWD ? launch(bias_softmax_bwd_rows<T, VEC, NV, WARPS, MASKED, EDGE, FULL>, pl, s)
+             : launch(bias_softmax_fwd_rows<T, VEC, NV, WARPS, MASKED, EDGE, FULL>, pl, s);
+}
 template <typename T, int VEC, int NV, int WARPS, bool BWD, bool MASKED>
 int launch_rows(const Plan& pl, cudaStream_t s) {
-  if (pl.edge)
-    return BWD ? launch(bias_softmax_bwd_rows<T, VEC, NV, WARPS, MASKED, true>, pl, s) : launch(bias_softmax_fwd_rows<T, VEC, NV, WARPS, MASKED, true>, pl, s);
-  return BWD ? launch(bias_softmax_bwd_rows<T, VEC, NV, WARPS, MASKED, false>, pl, s) : launch(bias_softmax_fwd_rows<T, VEC, NV, WARPS, MASKED, false>, pl, s);
+  if (pl.full) return launch_row<T, VEC, NV, WARPS, MASKED, false, true, BWD>(pl, s);
+  if (pl.edge) return launch_row<T, VEC, NV, WARPS, MASKED, true, false, BWD>(pl, s);
+  return launch_row<T, VEC, NV, WARPS, MASKED, false, false, BWD>(pl, s);
 }
 template <typename T, int VEC, bool BWD, bool MASKED>
 int dispatch(const Plan& pl, cudaStream_t s) {

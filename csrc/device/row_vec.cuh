@@ -19,6 +19,14 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return
 // N elements that start on a boundary of their own size (at most 16 bytes): one load or store instruction.
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
 
+// Asynchronous copies of 16 bytes to shared memory; a thread waits for its own.
+__device__ __forceinline__ void copy16_async(void* shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(shared)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+
 template <typename T, int N>
 __device__ __forceinline__ void load(const T* __restrict__ p, float (&out)[N]) {
   const Pack<T, N> raw = *reinterpret_cast<const Pack<T, N>*>(p);

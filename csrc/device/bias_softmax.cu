@@ -13,7 +13,6 @@
 // for every group of lanes that walks over rows of its own.  In one row no two elements have the same distance, so no atomics
 // are needed and the order of every sum is fixed: the same inputs give the same bits.
 #include "kernels_api.h"
-#include <cstdlib>
 #include "row_vec.cuh"
 
 namespace {
@@ -706,8 +705,8 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
   int resident = (bwd ? 768 : 1024) / pl.threads;
   const int by_smem = (int)(220 * 1024 / (pl.smem + 1536));
   if (resident > by_smem) resident = by_smem > 0 ? by_smem : 1;
-  static const int mult = getenv("CB_M") ? atoi(getenv("CB_M")) : 1;
-  long long blocks = 148LL * resident * mult / (p.H > 0 ? p.H : 1);
+  
+  long long blocks = 148LL * resident / (p.H > 0 ? p.H : 1);
   const long long most = ((long long)a.rows + groups - 1) / groups;
   if (blocks > most) blocks = most;
   if (blocks < 1) blocks = 1;

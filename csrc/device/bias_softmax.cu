@@ -65,13 +65,16 @@ __device__ __forceinline__ int bucket_of(int rel, const B200RelativeBuckets& rb)
 // One pad word every 32: lanes that read eight neighbours each then meet in different banks.
 __host__ __device__ __forceinline__ int padded(int x) { return x + (x >> 5); }
 
-// Words of shared memory in front of the rows on their way, which begin on a 16-byte boundary.
-__host__ __device__ __forceinline__ int ring_offset(int last) { return (padded(last) + 1 + 3) & ~3; }
-__host__ __device__ __forceinline__ int ring_offset_bwd(int last, int groups) { return ((groups + 1) * (padded(last) + 1) + 3) & ~3; }
+// Words of shared memory: the table of biases, the sums over distances of every group; the rows on their way begin behind them on a
+// 16-byte boundary.
+__host__ __device__ __forceinline__ int lut_words(int last) { return (padded(last) + 1 + 3) & ~3; }
+__host__ __device__ __forceinline__ int acc_words(int last, int groups) { return (groups * (padded(last) + 1) + 3) & ~3; }
 
+// Called by the whole block; ends with a barrier.
 __device__ __forceinline__ void fill_lut(float* lut, const Args& p, int h) {
   for (int x = threadIdx.x; x <= p.last; x += blockDim.x)
     lut[padded(x)] = scalar_at(p.table, (long long)bucket_of(x - p.reach, p.rb) * p.H + h, p.table_dtype);
+  __syncthreads();
 }
 
 // Vectors of VEC elements (16 bytes) on 16-byte boundaries.  EDGE: rows may begin anywhere and have any length, so that the
@@ -97,18 +100,47 @@ __device__ __forceinline__ void store_part(T* row, int j0, int n, const Pack<T, 
   }
 }
 
-__device__ __forceinline__ float2 masked(float2 a, float2 m) {
-  return make_float2(m.x == kNegInf ? kNegInf : a.x + m.x, m.y == kNegInf ? kNegInf : a.y + m.y);
+// Adds a vector of the mask; excluded elements become -inf whatever they held, NaN too.  Returns whether there are any.  Most vectors
+// of most masks (padding, causal) are all 0 or all -inf, which takes a few tests on their bits instead of four instructions an element.
+__device__ __forceinline__ bool add_mask_pair(float2& a, float2 m) {
+  const bool x = m.x == kNegInf, y = m.y == kNegInf;
+  a = make_float2(x ? kNegInf : a.x + m.x, y ? kNegInf : a.y + m.y);
+  return x || y;
 }
+template <int N>
+__device__ __forceinline__ bool exclude_all(float2 (&a)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) a[k] = both(kNegInf);
+  return true;
+}
+template <typename M> __device__ __forceinline__ unsigned neg_inf_word();
+template <> __device__ __forceinline__ unsigned neg_inf_word<float>() { return 0xff800000u; }
+template <> __device__ __forceinline__ unsigned neg_inf_word<__nv_bfloat16>() { return 0xff80ff80u; }
+template <> __device__ __forceinline__ unsigned neg_inf_word<__half>() { return 0xfc00fc00u; }
 template <typename M, int VEC>
-__device__ __forceinline__ void add_mask_vector(const M* m, float2 (&a)[VEC / 2]) {
-  constexpr int W = 16 / sizeof(M) < VEC ? 16 / sizeof(M) : VEC;
+__device__ __forceinline__ bool add_mask_vector(const M* m, float2 (&a)[VEC / 2]) {
+  constexpr int W = 16 / sizeof(M) < VEC ? 16 / sizeof(M) : VEC, P = VEC / W, WORDS = sizeof(Pack<M, W>) / 4;
+  Pack<M, W> part[P];
+  unsigned any = 0, other = 0;
 #pragma unroll
-  for (int o = 0; o < VEC; o += W) {
-    const Pack<M, W> part = *reinterpret_cast<const Pack<M, W>*>(m + o);
+  for (int o = 0; o < P; ++o) {
+    part[o] = *reinterpret_cast<const Pack<M, W>*>(m + o * W);
+    const unsigned* w = reinterpret_cast<const unsigned*>(&part[o]);
 #pragma unroll
-    for (int k = 0; k < W / 2; ++k) a[o / 2 + k] = masked(a[o / 2 + k], pair_of(part, k));
+    for (int k = 0; k < WORDS; ++k) {
+      any |= w[k];
+      other |= w[k] ^ neg_inf_word<M>();
+    }
   }
+  if (any == 0) return false;
+  if (other == 0) return exclude_all(a);
+  bool out = false;
+#pragma unroll
+  for (int o = 0; o < P; ++o) {
+#pragma unroll
+    for (int k = 0; k < W / 2; ++k) out |= add_mask_pair(a[o * W / 2 + k], pair_of(part[o], k));
+  }
+  return out;
 }
 
 // The mask of one row: where key 0 has its element, and whether the row's vectors lie on the boundaries of wide loads.
@@ -126,34 +158,43 @@ __device__ __forceinline__ MaskRow mask_row(const Args& p, long long at, int pha
   return m;
 }
 
-// Adds the mask to the scores of [j0, j0 + VEC); excluded elements become -inf whatever they held, NaN too.
+// Adds the mask to the scores of [j0, j0 + VEC).  Returns whether it excludes any.
 template <int VEC, bool EDGE>
-__device__ __forceinline__ void add_mask(const Args& p, const MaskRow& row, int j0, float2 (&a)[VEC / 2]) {
+__device__ __forceinline__ bool add_mask(const Args& p, const MaskRow& row, int j0, float2 (&a)[VEC / 2]) {
   if (row.wide && (!EDGE || (j0 >= 0 && j0 + VEC <= p.Lk))) {
     const char* m = row.key0 + j0 * mask_bytes(p.mask_dtype);
-    if (p.mask_dtype == B200_F32) add_mask_vector<float, VEC>(reinterpret_cast<const float*>(m), a);
-    else if (p.mask_dtype == B200_BF16) add_mask_vector<__nv_bfloat16, VEC>(reinterpret_cast<const __nv_bfloat16*>(m), a);
-    else if (p.mask_dtype == B200_F16) add_mask_vector<__half, VEC>(reinterpret_cast<const __half*>(m), a);
-    else {
-      const Pack<unsigned char, VEC> keep = *reinterpret_cast<const Pack<unsigned char, VEC>*>(m);
-#pragma unroll
-      for (int k = 0; k < VEC / 2; ++k) a[k] = make_float2(keep.v[2 * k] ? a[k].x : kNegInf, keep.v[2 * k + 1] ? a[k].y : kNegInf);
+    if (p.mask_dtype == B200_F32) return add_mask_vector<float, VEC>(reinterpret_cast<const float*>(m), a);
+    if (p.mask_dtype == B200_BF16) return add_mask_vector<__nv_bfloat16, VEC>(reinterpret_cast<const __nv_bfloat16*>(m), a);
+    if (p.mask_dtype == B200_F16) return add_mask_vector<__half, VEC>(reinterpret_cast<const __half*>(m), a);
+    const Pack<unsigned char, VEC> keep = *reinterpret_cast<const Pack<unsigned char, VEC>*>(m);
+    const unsigned* w = reinterpret_cast<const unsigned*>(&keep);
+    unsigned kept = w[0], any = w[0];
+    if (VEC == 8) {
+      kept &= w[VEC / 4 - 1];
+      any |= w[VEC / 4 - 1];
     }
-    return;
+    if (kept == 0x01010101u) return false;
+    if (any == 0) return exclude_all(a);
+#pragma unroll
+    for (int k = 0; k < VEC / 2; ++k) a[k] = make_float2(keep.v[2 * k] ? a[k].x : kNegInf, keep.v[2 * k + 1] ? a[k].y : kNegInf);
+    return true;
   }
+  bool out = false;
 #pragma unroll
   for (int k = 0; k < VEC / 2; ++k) {
     const int j = j0 + 2 * k;
     float2 m = make_float2(0.f, 0.f);
     if (j >= 0 && j < p.Lk) m.x = scalar_at(row.key0, j * p.mk_j, p.mask_dtype);
     if (j + 1 >= 0 && j + 1 < p.Lk) m.y = scalar_at(row.key0, (j + 1) * p.mk_j, p.mask_dtype);
-    a[k] = masked(a[k], m);
+    out |= add_mask_pair(a[k], m);
   }
+  return out;
 }
 
-// Scores to logits: scale, bias by distance, mask; -inf outside the row.  x0 = slot of the first element's distance.
+// Scores to logits: scale, bias by distance, mask; -inf outside the row.  x0 = slot of the first element's distance.  Returns
+// whether any element is excluded.
 template <typename T, int VEC, bool MASKED, bool EDGE>
-__device__ __forceinline__ void to_logits(const Args& p, const float* lut, const MaskRow& mask, int j0, int x0, const Pack<T, VEC>& s, float2 (&a)[VEC / 2]) {
+__device__ __forceinline__ bool to_logits(const Args& p, const float* lut, const MaskRow& mask, int j0, int x0, const Pack<T, VEC>& s, float2 (&a)[VEC / 2]) {
   const int last = p.last;
   const float2 scale = both(p.scale);
   if (x0 >= last || x0 + VEC - 1 <= 0) {  // all as far as the bias tells apart
@@ -167,8 +208,10 @@ __device__ __forceinline__ void to_logits(const Args& p, const float* lut, const
       a[k] = fma2(pair_of(s, k), scale, make_float2(lut[padded(min(max(x, 0), last))], lut[padded(min(max(x + 1, 0), last))]));
     }
   }
-  if (MASKED) add_mask<VEC, EDGE>(p, mask, j0, a);
+  bool out = false;
+  if (MASKED) out = add_mask<VEC, EDGE>(p, mask, j0, a);
   if (EDGE && (j0 < 0 || j0 + VEC > p.Lk)) {
+    out = true;
 #pragma unroll
     for (int k = 0; k < VEC / 2; ++k) {
       const int j = j0 + 2 * k;
@@ -176,6 +219,7 @@ __device__ __forceinline__ void to_logits(const Args& p, const float* lut, const
       if (j + 1 < 0 || j + 1 >= p.Lk) a[k].y = kNegInf;
     }
   }
+  return out;
 }
 
 // e^(a - m).  The difference comes first: a and m may be as large as the type allows (a mask of its lowest value on a whole row).
@@ -309,7 +353,7 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
   using Vectors = RowVectors<T, VEC, NV, EDGE, FULL>;
   constexpr int kDepth = ring_depth(NV, false);
   const T* base = static_cast<const T*>(p.s);
-  Pack<T, VEC>* ring = reinterpret_cast<Pack<T, VEC>*>(lut + ring_offset(p.last)) + threadIdx.x;
+  Pack<T, VEC>* ring = reinterpret_cast<Pack<T, VEC>*>(lut + lut_words(p.last)) + threadIdx.x;
   RowWalk row(p, min(r, p.rows - 1), h), ahead = row;  // a group behind the last row follows on rows that are there
   unsigned fetched = 0;
   auto fetch_next = [&](int stage) {
@@ -323,7 +367,6 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
 #pragma unroll
   for (int d = 0; d < kDepth - 1; ++d) fetch_next(d);
   fill_lut(lut, p, h);
-  __syncthreads();
   int turn = 0, stage = 0;
   for (unsigned done = 0; r0 + done < r1; done += groups, turn ^= 1) {
     const bool live = r + done < r1;
@@ -423,7 +466,7 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
   const int h = blockIdx.x / p.blocks_per_head, part = blockIdx.x % p.blocks_per_head;
   const int G = WARPS == 1 ? p.group : 32, lanes = G * WARPS;
   const int gl = WARPS == 1 ? threadIdx.x & (G - 1) : threadIdx.x, groups = WARPS == 1 ? blockDim.x / G : 1;
-  float* all = lut + words;
+  float* all = lut + lut_words(p.last);
   float* acc = all + (WARPS == 1 ? (threadIdx.x / G) * words : 0);
   float below = 0.f, above = 0.f;
   const unsigned r0 = part * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
@@ -432,7 +475,7 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
   constexpr int kDepth = ring_depth(NV, true);
   const T* base = static_cast<const T*>(p.s);
   const T* gbase = static_cast<const T*>(p.g);
-  Pack<T, VEC>* ring = reinterpret_cast<Pack<T, VEC>*>(lut + ring_offset_bwd(p.last, groups)) + threadIdx.x;
+  Pack<T, VEC>* ring = reinterpret_cast<Pack<T, VEC>*>(lut + lut_words(p.last) + acc_words(p.last, groups)) + threadIdx.x;
   RowWalk row(p, min(r, p.rows - 1), h), ahead = row;
   unsigned fetched = 0;
   auto fetch_next = [&](int stage) {
@@ -447,10 +490,9 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
 #pragma unroll
   for (int d = 0; d < kDepth - 1; ++d) fetch_next(d);
   float2 st_next = p.stats[row.stat];
-  fill_lut(lut, p, h);
   if (p.partial)
     for (int x = threadIdx.x; x < groups * words; x += blockDim.x) all[x] = 0.f;
-  __syncthreads();
+  fill_lut(lut, p, h);
   int turn = 0, stage = 0;
   for (unsigned done = 0; r0 + done < r1; done += groups, turn ^= 1) {
     const bool live = r + done < r1;
@@ -470,18 +512,22 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
     const MaskRow mask = MASKED ? mask_row<VEC>(p, now.mask, phase) : MaskRow{};
     const int first_x = now.first_x(p);
     float2 a[NV][VEC / 2], dot2 = make_float2(0.f, 0.f);
+    int excluded = 0;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int j0 = (gl + n * lanes) * VEC - phase;
       if (FULL || j0 < p.Lk) {
-        to_logits<T, VEC, MASKED, EDGE>(p, lut, mask, j0, first_x + j0, raw[n], a[n]);
+        const bool out = to_logits<T, VEC, MASKED, EDGE>(p, lut, mask, j0, first_x + j0, raw[n], a[n]);
 #pragma unroll
-        for (int k = 0; k < VEC / 2; ++k) {
-          a[n][k] = mul2(weights_of(a[n][k], both(-st.x)), both(st.y));
-          float2 g2 = pair_of(graw[n], k);
-          if (MASKED || EDGE) g2 = make_float2(a[n][k].x == 0.f ? 0.f : g2.x, a[n][k].y == 0.f ? 0.f : g2.y);  // an excluded key counts nothing
-          dot2 = fma2(a[n][k], g2, dot2);
+        for (int k = 0; k < VEC / 2; ++k) a[n][k] = mul2(weights_of(a[n][k], both(-st.x)), both(st.y));
+        if ((MASKED || EDGE) && out) {  // an excluded key counts nothing, whatever its gradient holds
+          excluded |= 1 << n;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k)
+            if ((k % 2 ? a[n][k / 2].y : a[n][k / 2].x) == 0.f) graw[n].v[k] = from_f32<T>(0.f);
         }
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k) dot2 = fma2(a[n][k], pair_of(graw[n], k), dot2);
       }
     }
     // (with its barrier this row's sums over distances come behind the last row's)
@@ -494,10 +540,10 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
         if (FULL || j0 < p.Lk) {
 #pragma unroll
           for (int k = 0; k < VEC / 2; ++k) {
-            float2 d = mul2(a[n][k], add2(pair_of(graw[n], k), dot));
-            if (MASKED || EDGE) d = make_float2(a[n][k].x == 0.f ? 0.f : d.x, a[n][k].y == 0.f ? 0.f : d.y);
-            a[n][k] = d;
-            set_pair(raw[n], k, mul2(d, both(p.scale)));
+            const float2 d = mul2(a[n][k], add2(pair_of(graw[n], k), dot));
+            if ((MASKED || EDGE) && (excluded >> n & 1)) a[n][k] = make_float2(a[n][k].x == 0.f ? 0.f : d.x, a[n][k].y == 0.f ? 0.f : d.y);
+            else a[n][k] = d;
+            set_pair(raw[n], k, mul2(a[n][k], both(p.scale)));
           }
           store_part<T, VEC, EDGE>(o, j0, p.Lk, raw[n]);
           if (p.partial) add_distances<VEC>(acc, p.last, first_x + j0, a[n], below, above);
@@ -528,7 +574,6 @@ __global__ void __launch_bounds__(kMaxThreads) bias_softmax_fwd_long(const __gri
   __shared__ float sh[32];
   const int h = blockIdx.x / p.blocks_per_head, part = blockIdx.x % p.blocks_per_head;
   fill_lut(lut, p, h);
-  __syncthreads();
   const unsigned r0 = part * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
   RowWalk walk(p, r0, h);
   for (unsigned r = r0; r < r1; ++r, walk.advance(p, 1)) {
@@ -571,11 +616,10 @@ __global__ void __launch_bounds__(kMaxThreads) bias_softmax_bwd_long(const __gri
   __shared__ float sh[32];
   const int words = padded(p.last) + 1;
   const int h = blockIdx.x / p.blocks_per_head, part = blockIdx.x % p.blocks_per_head;
-  float* acc = lut + words;
-  fill_lut(lut, p, h);
+  float* acc = lut + lut_words(p.last);
   if (p.partial)
     for (int x = threadIdx.x; x < words; x += blockDim.x) acc[x] = 0.f;
-  __syncthreads();
+  fill_lut(lut, p, h);
   float below = 0.f, above = 0.f;
   const unsigned r0 = part * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
   RowWalk walk(p, r0, h);
@@ -698,9 +742,8 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
     pl.threads = 32 * pl.warps;
   }
   pl.full = aligned && nvec == pl.nv * (pl.warps == 1 ? a.group : pl.threads);
-  pl.smem = (size_t)(bwd ? groups + 1 : 1) * words * 4;
-  if (pl.nv)
-    pl.smem = (bwd ? ring_offset_bwd(a.last, groups) : ring_offset(a.last)) * 4 + (size_t)ring_depth(pl.nv, bwd) * pl.nv * pl.threads * 16 * (bwd ? 2 : 1);
+  pl.smem = (size_t)lut_words(a.last) * 4 + (bwd ? acc_words(a.last, groups) * 4 : 0) +
+            (size_t)(pl.nv ? ring_depth(pl.nv, bwd) * pl.nv * pl.threads * 16 * (bwd ? 2 : 1) : 0);
   // One wave of blocks: each has to build its table of biases first, and what it leaves for the table gradient has to be added up.
   int resident = (bwd ? 768 : 1024) / pl.threads;
   const int by_smem = (int)(220 * 1024 / (pl.smem + 1536));

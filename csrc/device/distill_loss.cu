@@ -17,22 +17,28 @@ namespace {
 using namespace rowvec;
 
 constexpr float kNegInf = -__builtin_huge_valf();
-constexpr int kThreads = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxThreads = 512;
+constexpr int kUnroll = 4;  // vectors under way in each thread
 
 struct Shared {
-  float red[32];
-  int idx[B200_DISTILL_MAX_K];
-  float share[B200_DISTILL_MAX_K];
+  float2 student[kMaxThreads / 32], teacher[kMaxThreads / 32];  // each warp's (maximum, sum of exponentials)
+  float loss[kMaxThreads / 32];
+  __align__(16) int idx[B200_DISTILL_MAX_K];
+  __align__(16) float share[B200_DISTILL_MAX_K];
+  int last;
 };
 
-__device__ __forceinline__ float warp_red(float v, bool is_max) { return is_max ? group_max(v, 32) : group_sum(v, 32); }
-__device__ __forceinline__ float block_red(float v, bool is_max, float* sh) {
-  v = warp_red(v, is_max);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = warp_red((threadIdx.x & 31) < blockDim.x / 32 ? sh[threadIdx.x & 31] : (is_max ? kNegInf : 0.f), is_max);
-  __syncthreads();
-  return v;
+__device__ __forceinline__ float finite_max(float m) { return m == kNegInf ? 0.f : m; }
+// The pairs of 32 lanes, then of a block's warps, as one: (maximum, sum of the exponentials of c times the distance to it).
+__device__ __forceinline__ float2 join(float m, float s, float c) {
+  const float top = group_max(m, 32);
+  return make_float2(top, group_sum(s * exp2_fast((m - finite_max(top)) * c), 32));  // m = -inf: nothing, or a NaN
+}
+__device__ __forceinline__ float2 join_warps(const float2* sh, float c) {
+  const int lane = threadIdx.x & 31;
+  const float2 v = lane < blockDim.x / 32 ? sh[lane] : make_float2(kNegInf, 0.f);
+  return join(v.x, v.y, c);
 }
 
 __device__ __forceinline__ float teacher_at(const void* p, long long i, int dt) {
@@ -50,114 +56,199 @@ __device__ __forceinline__ bool present(const B200Distill& p, long long row, int
   return i >= 0 && i < p.V && teacher_at(p.teacher, row * p.teacher_ld + k, p.teacher_dtype) != kNegInf;
 }
 
-// Loads the row's entries into shared memory: indices (-1: absent) and shares.  Returns whether there are any; *plogp: this
-// thread's part of sum p log p.
-__device__ __forceinline__ bool load_teacher(const B200Distill& p, long long row, Shared& sh, float* plogp) {
-  float top = kNegInf;
-  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
-    const long long i = index_at(p, row, k);
-    const float t = teacher_at(p.teacher, row * p.teacher_ld + k, p.teacher_dtype);
-    const bool there = i >= 0 && i < p.V && t != kNegInf;
-    if (i >= p.V && p.bad_flag) *p.bad_flag = 1;
-    sh.idx[k] = there ? (int)i : -1;
-    sh.share[k] = t;
-    if (there) top = fmaxf(top, t);
+// A kept entry of the row in work: each thread has up to two.
+struct Entry {
+  int idx;      // -1: absent
+  float value;  // the teacher's logit, then its share
+  float z;      // the student's logit
+};
+
+// A row: `head` elements up to the first 16-byte boundary, whole vectors, `tail` elements.
+template <typename T, int VEC>
+struct Row {
+  const T* z;
+  int head, tail;
+  unsigned vectors;
+  __device__ __forceinline__ Row(const T* p, int V) : z(p) {
+    head = (int)((VEC - ((reinterpret_cast<uintptr_t>(p) / sizeof(T)) & (VEC - 1))) & (VEC - 1));
+    if (head > V) head = V;
+    vectors = (unsigned)(V - head) / VEC;
+    tail = (V - head) % VEC;
   }
-  int any = 0;
-  for (int k = threadIdx.x; k < p.K; k += blockDim.x) any |= sh.idx[k] >= 0;
-  any = __syncthreads_or(any);
-  top = block_red(top, true, sh.red);
-  float sum = 0.f;
-  for (int k = threadIdx.x; k < p.K; k += blockDim.x)
-    if (sh.idx[k] >= 0) sum += __expf((sh.share[k] - top) * p.inv_temperature);
-  sum = block_red(sum, false, sh.red);
-  const float logsum = logf(sum);
-  float part = 0.f;
-  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
-    if (sh.idx[k] < 0) continue;
-    const float lp = (sh.share[k] - top) * p.inv_temperature - logsum, share = expf(lp);
-    sh.share[k] = share;
-    part += share == 0.f ? 0.f : share * lp;
-  }
-  *plogp = part;
-  __syncthreads();
-  return any != 0;
-}
+  __device__ __forceinline__ int ragged(int e, int V) const { return e < head ? e : V - tail + e - head; }  // place of ragged element e
+};
 
 template <typename T, int VEC, bool FWD, bool GRAD>
-__global__ void __launch_bounds__(kThreads) distill_kernel(const __grid_constant__ B200Distill p) {
+__global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_constant__ B200Distill p) {
   __shared__ Shared sh;
-  // the factor of the gradient: what backward() was given, over the number of rows for a mean
-  float count_inv = 1.f;
-  if (GRAD && p.count) count_inv = 1.f / fmaxf(*p.count, 1.f);
   if (GRAD && !FWD && p.skip_factor_one && *p.grad == 1.f) return;  // the forward has written this gradient
-  const float c = p.inv_temperature * 1.4426950408889634f;
+  const int V = (int)p.V, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float c = p.inv_temperature * kLog2e;
+  float count_inv = GRAD && !FWD && p.count ? 1.f / fmaxf(*p.count, 1.f) : 1.f;
+  bool counted = false;
   for (long long row = blockIdx.x; row < p.N; row += gridDim.x) {
-    const T* z = static_cast<const T*>(p.logits) + row * p.ld;
-    const int phase = (int)((reinterpret_cast<uintptr_t>(z) / sizeof(T)) & (VEC - 1));
-    float plogp;
-    const bool any = load_teacher(p, row, sh, &plogp);
+    const Row<T, VEC> r(static_cast<const T*>(p.logits) + row * p.ld, V);
+    const T* body = r.z + r.head;
+    // the row's kept entries come in while the logits are read
+    Entry e[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int k = threadIdx.x + q * blockDim.x;
+      e[q].idx = -1;
+      if (k < p.K) {
+        const long long i = index_at(p, row, k);
+        e[q].value = teacher_at(p.teacher, row * p.teacher_ld + k, p.teacher_dtype);
+        if (i >= 0 && i < p.V) e[q].idx = (int)i;
+        else if (i >= p.V && p.bad_flag) *p.bad_flag = 1;
+      }
+    }
     float m, s;
     if (FWD) {
       m = kNegInf;
       s = 0.f;
-      for (int j0 = (int)threadIdx.x * VEC - phase; j0 < p.V; j0 += kThreads * VEC) {
-        float v[VEC];
-        const bool whole = j0 >= 0 && j0 + VEC <= p.V;
-        if (whole) {
-          load<T, VEC>(z + j0, v);
-        } else {
+      for (unsigned v0 = threadIdx.x; v0 < r.vectors; v0 += kUnroll * blockDim.x) {
+        Pack<T, VEC> raw[kUnroll];
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) v[k] = j0 + k >= 0 && j0 + k < p.V ? to_f32<T>(z[j0 + k]) : kNegInf;
+        for (int u = 0; u < kUnroll; ++u)
+          if (v0 + u * blockDim.x < r.vectors) raw[u] = *reinterpret_cast<const Pack<T, VEC>*>(body + (size_t)(v0 + u * blockDim.x) * VEC);
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          if (v0 + u * blockDim.x < r.vectors) {
+#pragma unroll
+            for (int k = 0; k < VEC / 2; ++k) {
+              const float2 x = pair_of(raw[u], k);
+              top = fmaxf(top, fmaxf(x.x, x.y));
+            }
+          }
         }
-        float top = v[0];
-#pragma unroll
-        for (int k = 1; k < VEC; ++k) top = fmaxf(top, v[k]);
         if (top > m) {
-          s *= exp2f((m - top) * c);
+          s *= exp2_fast((m - top) * c);
           m = top;
         }
+        const float2 minus = both(-finite_max(m));
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) s += v[k] == kNegInf ? 0.f : exp2f((v[k] - m) * c);
+        for (int u = 0; u < kUnroll; ++u) {
+          if (v0 + u * blockDim.x < r.vectors) {
+#pragma unroll
+            for (int k = 0; k < VEC / 2; ++k) {
+              const float2 x = mul2(add2(pair_of(raw[u], k), minus), both(c));
+              sum = add2(sum, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
+            }
+          }
+        }
+        s += sum.x + sum.y;
       }
-      const float top = block_red(m, true, sh.red);
-      s = block_red(m == kNegInf ? s : s * exp2f((m - top) * c), false, sh.red);
-      m = top;
-      if (p.stats && threadIdx.x == 0) reinterpret_cast<float2*>(p.stats)[row] = make_float2(m, s);
-      const float logs = logf(s);
-      float part = plogp;
-      for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
-        if (sh.idx[k] < 0 || sh.share[k] == 0.f) continue;
-        part -= sh.share[k] * ((to_f32<T>(z[sh.idx[k]]) - m) * p.inv_temperature - logs);
+      for (int g = threadIdx.x; g < r.head + r.tail; g += blockDim.x) {
+        const float x = to_f32<T>(r.z[r.ragged(g, V)]);
+        if (x > m) {
+          s *= exp2_fast((m - x) * c);
+          m = x;
+        }
+        s += exp2_fast((x - finite_max(m)) * c);
       }
-      part = block_red(part, false, sh.red);
-      if (threadIdx.x == 0) p.row_loss[row] = any ? part * p.temperature * p.temperature : 0.f;
+      const float2 mine = join(m, s, c);
+      if (lane == 0) sh.student[warp] = mine;
     } else {
       const float2 st = reinterpret_cast<const float2*>(p.stats)[row];
       m = st.x;
       s = st.y;
     }
+    // the teacher's softmax, in the same way
+    float t_top = kNegInf, t_sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if (e[q].idx >= 0 && e[q].value == kNegInf) e[q].idx = -1;
+      if (e[q].idx >= 0) {
+        t_top = fmaxf(t_top, e[q].value);
+        e[q].z = to_f32<T>(r.z[e[q].idx]);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (e[q].idx >= 0) t_sum += exp2_fast((e[q].value - finite_max(t_top)) * c);
+    const float2 kept = join(t_top, t_sum, c);
+    if (lane == 0) sh.teacher[warp] = kept;
+    const bool any = __syncthreads_or(e[0].idx >= 0 || e[1].idx >= 0);
+    if (FWD) {
+      const float2 st = join_warps(sh.student, c);
+      m = finite_max(st.x);
+      s = st.y;
+      if (p.stats && threadIdx.x == 0) reinterpret_cast<float2*>(p.stats)[row] = make_float2(m, s);
+    }
+    const float2 t = join_warps(sh.teacher, c);
+    const float t_log = logf(t.y), s_log = FWD ? logf(s) : 0.f;
+    float part = 0.f;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int k = threadIdx.x + q * blockDim.x;
+      if (k >= p.K) continue;
+      if (e[q].idx >= 0) {
+        const float lp = (e[q].value - t.x) * p.inv_temperature - t_log;
+        e[q].value = expf(lp);
+        if (FWD && e[q].value != 0.f) part += e[q].value * (lp - ((e[q].z - m) * p.inv_temperature - s_log));
+      }
+      if (GRAD) {
+        sh.idx[k] = e[q].idx;
+        sh.share[k] = e[q].value;
+      }
+    }
+    if (FWD) {
+      part = group_sum(part, 32);
+      if (lane == 0) sh.loss[warp] = part;
+    }
+    __syncthreads();
+    if (FWD && warp == 0) {
+      part = group_sum(lane < blockDim.x / 32 ? sh.loss[lane] : 0.f, 32);
+      if (lane == 0) p.row_loss[row] = any ? part * p.temperature * p.temperature : 0.f;
+    }
     if (GRAD) {
-      T* d = static_cast<T*>(p.dlogits) + row * p.ld;
-      const float factor = any ? (FWD ? 1.f : p.grad[p.grad_per_row ? row * p.grad_ld : 0]) * count_inv * p.temperature : 0.f;
-      const float scale = factor / s;
-      for (int j0 = (int)threadIdx.x * VEC - phase; j0 < p.V; j0 += kThreads * VEC) {
-        float v[VEC];
-        if (j0 >= 0 && j0 + VEC <= p.V) {
-          load<T, VEC>(z + j0, v);
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) v[k] = any ? scale * exp2f((v[k] - m) * c) : 0.f;
-          store<T, VEC>(d + j0, v);
-        } else {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k)
-            if (j0 + k >= 0 && j0 + k < p.V) d[j0 + k] = from_f32<T>(any ? scale * exp2f((to_f32<T>(z[j0 + k]) - m) * c) : 0.f);
+      if (FWD && !counted) {  // the number of rows comes from the kernel in front, which may still run
+        if (p.count) {
+          cudaGridDependencySynchronize();
+          count_inv = 1.f / fmaxf(*static_cast<volatile const float*>(p.count), 1.f);
         }
+        counted = true;
+      }
+      T* d = static_cast<T*>(p.dlogits) + row * p.ld;
+      T* d_body = d + r.head;
+      const float factor = any ? (FWD ? 1.f : p.grad[p.grad_per_row ? row * p.grad_ld : 0]) * count_inv * p.temperature : 0.f;
+      const float scale = any ? factor / s : 0.f;
+      if (any) {
+        const float2 minus = both(-m);
+        for (unsigned v0 = threadIdx.x; v0 < r.vectors; v0 += kUnroll * blockDim.x) {
+          Pack<T, VEC> raw[kUnroll];
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u)
+            if (v0 + u * blockDim.x < r.vectors) raw[u] = *reinterpret_cast<const Pack<T, VEC>*>(body + (size_t)(v0 + u * blockDim.x) * VEC);
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u) {
+            if (v0 + u * blockDim.x < r.vectors) {
+#pragma unroll
+              for (int k = 0; k < VEC / 2; ++k) {
+                const float2 x = mul2(add2(pair_of(raw[u], k), minus), both(c));
+                set_pair(raw[u], k, mul2(make_float2(exp2_fast(x.x), exp2_fast(x.y)), both(scale)));
+              }
+              *reinterpret_cast<Pack<T, VEC>*>(d_body + (size_t)(v0 + u * blockDim.x) * VEC) = raw[u];
+            }
+          }
+        }
+      } else {
+        Pack<T, VEC> zero;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) zero.v[k] = from_f32<T>(0.f);
+        for (unsigned v = threadIdx.x; v < r.vectors; v += blockDim.x) *reinterpret_cast<Pack<T, VEC>*>(d_body + (size_t)v * VEC) = zero;
+      }
+      for (int g = threadIdx.x; g < r.head + r.tail; g += blockDim.x) {
+        const int j = r.ragged(g, V);
+        d[j] = from_f32<T>(any ? scale * exp2_fast((to_f32<T>(r.z[j]) - m) * c) : 0.f);
       }
       __syncthreads();
       // the kept entries: the first occurrence of an index writes the value with the shares of all of them
-      for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
-        const int i = sh.idx[k];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int k = threadIdx.x + q * blockDim.x, i = e[q].idx;
         if (i < 0) continue;
         bool first = true;
         float share = 0.f;
@@ -166,48 +257,88 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const __grid_constant
           first = first && o >= k;
           share += sh.share[o];
         }
-        if (first) d[i] = from_f32<T>(scale * exp2f((to_f32<T>(z[i]) - m) * c) - factor * share);
+        if (first) d[i] = from_f32<T>(scale * exp2_fast((e[q].z - m) * c) - factor * share);
       }
     }
-    __syncthreads();  // the next row overwrites the entries
+  }
+  if (!FWD || !p.loss) return;
+  // The block that ends last adds up the rows' losses, in an order that does not depend on which one it is.
+  cudaGridDependencySynchronize();  // the ticket was set by the kernel in front
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    sh.last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!sh.last) return;
+  float sum = 0.f;
+  for (long long i = threadIdx.x; i < p.N; i += blockDim.x) sum += __ldcg(p.row_loss + i);
+  sum = group_sum(sum, 32);
+  if (lane == 0) sh.loss[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0.f;
+    for (int w = 0; w < blockDim.x / 32; ++w) sum += sh.loss[w];
+    *p.loss = p.count ? sum / fmaxf(__ldcg(p.count), 1.f) : sum;
   }
 }
 
-// The number of rows with at least one entry.
+// The number of rows with at least one entry (for a mean), and the ticket of the blocks that follow.  One block: the kernel behind it
+// starts at once and needs the number only when its first gradients are written.
 __global__ void __launch_bounds__(1024) distill_count_kernel(const __grid_constant__ B200Distill p) {
-  __shared__ float red[32];
-  float n = 0.f;
+  cudaTriggerProgrammaticLaunchCompletion();
+  __shared__ int red[32];
+  if (threadIdx.x == 0) *p.ticket = 0;
+  if (!p.count) return;
+  int n = 0;
+#pragma unroll 4
   for (long long row = threadIdx.x; row < p.N; row += blockDim.x) {
-    int k = 0;
-    while (k < p.K && !present(p, row, k)) ++k;
-    n += k < p.K ? 1.f : 0.f;
+    bool there = false;
+    for (int k = 0; !there && k < p.K; ++k) there = present(p, row, k);
+    n += there;
   }
-  n = block_red(n, false, red);
-  if (threadIdx.x == 0) *p.count = n;
-}
-
-// Sum of the rows' losses over `count` (null: 1), in a fixed order.
-__global__ void __launch_bounds__(1024) distill_sum_kernel(const float* rows, long long n, const float* count, float* loss) {
-  __shared__ float red[32];
-  float s = 0.f;
-  for (long long i = threadIdx.x; i < n; i += blockDim.x) s += rows[i];
-  s = block_red(s, false, red);
-  if (threadIdx.x == 0) *loss = count ? s / fmaxf(*count, 1.f) : s;
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    n = __reduce_add_sync(0xffffffffu, red[threadIdx.x]);
+    if (threadIdx.x == 0) *p.count = (float)n;
+  }
 }
 
 bool valid(const B200Distill* p) {
   return p->N >= 0 && p->V >= 1 && p->V < (1LL << 31) - 8192 && p->K >= 0 && p->K <= B200_DISTILL_MAX_K && p->temperature > 0.f &&
-         (p->index_dtype == B200_I64 || p->index_dtype == B200_I32);
+         (p->index_dtype == B200_I64 || p->index_dtype == B200_I32) && (!p->loss || p->ticket);
 }
 
+// Threads for a row: about two rounds of unrolled vectors, and at least half as many as there are kept entries.
+int row_threads(const B200Distill& p) {
+  const long long vectors = p.V / (p.dtype == B200_F32 ? 4 : 8);
+  int t = 32;
+  while (t < kMaxThreads && (vectors > 2LL * kUnroll * t || p.K > 2 * t)) t *= 2;
+  return t;
+}
+
+// `after`: the counting kernel is in front and this one may begin before it ends.
 template <bool FWD, bool GRAD>
-int launch(const B200Distill& p, cudaStream_t s) {
-  const unsigned grid = (unsigned)(p.N < 148 * 4 ? p.N : 148 * 4);
-  if (p.dtype == B200_BF16) distill_kernel<__nv_bfloat16, 8, FWD, GRAD><<<grid, kThreads, 0, s>>>(p);
-  else if (p.dtype == B200_F16) distill_kernel<__half, 8, FWD, GRAD><<<grid, kThreads, 0, s>>>(p);
-  else if (p.dtype == B200_F32) distill_kernel<float, 4, FWD, GRAD><<<grid, kThreads, 0, s>>>(p);
-  else return (int)cudaErrorInvalidValue;
-  return (int)cudaGetLastError();
+int launch(const B200Distill& p, bool after, cudaStream_t s) {
+  const int threads = row_threads(p);
+  const long long most = 148LL * (2 * kMaxThreads / threads);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.N < most ? p.N : most));
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &overlap;
+  cfg.numAttrs = after ? 1 : 0;
+  cudaError_t e = cudaErrorInvalidValue;
+  if (p.dtype == B200_BF16) e = cudaLaunchKernelEx(&cfg, distill_kernel<__nv_bfloat16, 8, FWD, GRAD>, p);
+  else if (p.dtype == B200_F16) e = cudaLaunchKernelEx(&cfg, distill_kernel<__half, 8, FWD, GRAD>, p);
+  else if (p.dtype == B200_F32) e = cudaLaunchKernelEx(&cfg, distill_kernel<float, 4, FWD, GRAD>, p);
+  return (int)e;
 }
 
 }  // namespace
@@ -215,16 +346,16 @@ int launch(const B200Distill& p, cudaStream_t s) {
 extern "C" int b200_distill_fwd(const B200Distill* p, void* stream) {
   if (!valid(p)) return (int)cudaErrorInvalidValue;
   cudaStream_t s = (cudaStream_t)stream;
-  if (p->count) distill_count_kernel<<<1, 1024, 0, s>>>(*p);
-  if (p->N > 0) {
-    const int rc = p->dlogits ? launch<true, true>(*p, s) : launch<true, false>(*p, s);
+  if (p->N == 0) return p->loss ? (int)cudaMemsetAsync(p->loss, 0, sizeof(float), s) : 0;
+  if (p->loss) {
+    distill_count_kernel<<<1, 1024, 0, s>>>(*p);
+    const int rc = (int)cudaGetLastError();
     if (rc) return rc;
   }
-  if (p->loss) distill_sum_kernel<<<1, 1024, 0, s>>>(p->row_loss, p->N, p->count, p->loss);
-  return (int)cudaGetLastError();
+  return p->dlogits ? launch<true, true>(*p, p->loss != nullptr, s) : launch<true, false>(*p, p->loss != nullptr, s);
 }
 
 extern "C" int b200_distill_bwd(const B200Distill* p, void* stream) {
   if (!valid(p)) return (int)cudaErrorInvalidValue;
-  return p->N > 0 ? launch<false, true>(*p, (cudaStream_t)stream) : 0;
+  return p->N > 0 ? launch<false, true>(*p, false, (cudaStream_t)stream) : 0;
 }

@@ -656,13 +656,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> distill_fwd(const DistillArgs& a, boo
   }
   OpScope scope("top_logits_distillation", a.logits);
   Tensor z = row_layout(a.logits), teacher = a.teacher.contiguous(), index = a.index.contiguous();
-  Tensor rows = at::empty({N}, fopt), stats = at::empty({N, 2}, fopt), count = at::empty({1}, fopt);
+  Tensor rows = at::empty({N}, fopt), stats = at::empty({N, 2}, fopt), count = at::empty({2}, fopt);  // (count, scratch)
   Tensor loss = each ? rows : at::empty({}, fopt), grad;
   B200Distill p = distill_params(a, z, teacher, index);
   p.row_loss = rows.data_ptr<float>();
   p.stats = stats.data_ptr<float>();
   p.loss = each ? nullptr : loss.data_ptr<float>();
   p.count = mean ? count.data_ptr<float>() : nullptr;
+  p.ticket = reinterpret_cast<unsigned*>(count.data_ptr<float>() + 1);
   // The gradient for a factor of 1, while the row is in the caches.  Not in half precision: its training scales the loss, so that the
   // factor is another one, and a gradient rounded before the scaling would lose what the scaling is there to keep.
   if (need_grad && !each && z.scalar_type() != at::kHalf) {
@@ -683,7 +684,7 @@ Tensor distill_bwd(const DistillArgs& a, const Tensor& grad, const Tensor& stats
   TORCH_CHECK(each ? (grad.dim() == 1 && grad.size(0) == N) : grad.numel() == 1, op, ": the gradient has the shape of the loss, got ",
               grad.sizes());
   TORCH_CHECK(stats.dim() == 2 && stats.size(0) == N && stats.size(1) == 2 && stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
-                  count.numel() == 1 && count.scalar_type() == at::kFloat,
+                  count.numel() >= 1 && count.scalar_type() == at::kFloat,
               op, ": statistics are the forward's");
   check_same_device(op, a.logits, grad, stats, count);
   if (!on_device(a.logits))

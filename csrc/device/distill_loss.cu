@@ -19,7 +19,8 @@ using namespace rowvec;
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxThreads = 512;
-constexpr int kUnroll = 4;  // vectors under way in each thread
+constexpr int kUnit = 4;   // vectors that a thread takes at a time: a unit of a row is kUnit vectors for each thread
+constexpr int kDepth = 3;  // units under way
 
 struct Shared {
   float2 student[kMaxThreads / 32], teacher[kMaxThreads / 32];  // each warp's (maximum, sum of exponentials)
@@ -78,17 +79,71 @@ struct Row {
   __device__ __forceinline__ int ragged(int e, int V) const { return e < head ? e : V - tail + e - head; }  // place of ragged element e
 };
 
+// The units that a block will take, in order: a row's once for its sum, again for its gradient (then out of L2), then the next row's.
+// Each thread copies its vectors of the units to come to a place of its own in shared memory, so that reading never stops: not at a
+// row's reductions nor while its gradient is written.
+template <typename T, int VEC, int PASSES>
+struct Stream {
+  const B200Distill& p;
+  Pack<T, VEC>* ring;  // this thread's first vector; unit d begins at d * kUnit * blockDim
+  long long row;
+  int pass, put, got;
+  unsigned at, vectors;
+  const T* body;
+  __device__ __forceinline__ Stream(const B200Distill& args, void* shared)
+      : p(args), ring(static_cast<Pack<T, VEC>*>(shared) + threadIdx.x), row(blockIdx.x), pass(0), put(0), got(0), at(0) {
+    enter();
+#pragma unroll
+    for (int d = 0; d < kDepth - 1; ++d) next();
+  }
+  __device__ __forceinline__ void enter() {
+    if (row >= p.N) return;
+    const Row<T, VEC> r(static_cast<const T*>(p.logits) + row * p.ld, (int)p.V);
+    body = r.z + r.head;
+    vectors = r.vectors;
+  }
+  __device__ __forceinline__ void next() {
+    if (row < p.N) {
+#pragma unroll
+      for (int u = 0; u < kUnit; ++u) {
+        const unsigned v = at + u * blockDim.x + threadIdx.x;
+        if (v < vectors) copy16_async(ring + (put * kUnit + u) * blockDim.x, body + (size_t)v * VEC);
+      }
+      at += kUnit * blockDim.x;
+      if (at >= vectors) {
+        at = 0;
+        if (++pass == PASSES) {
+          pass = 0;
+          row += gridDim.x;
+          enter();
+        }
+      }
+    }
+    copies_commit();
+    put = put == kDepth - 1 ? 0 : put + 1;
+  }
+  __device__ __forceinline__ void take(Pack<T, VEC> (&raw)[kUnit]) {
+    next();
+    copies_wait<kDepth - 1>();
+#pragma unroll
+    for (int u = 0; u < kUnit; ++u) raw[u] = ring[(got * kUnit + u) * blockDim.x];
+    got = got == kDepth - 1 ? 0 : got + 1;
+  }
+};
+
 template <typename T, int VEC, bool FWD, bool GRAD>
 __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_constant__ B200Distill p) {
   __shared__ Shared sh;
+  extern __shared__ __align__(16) unsigned char ring[];
   if (GRAD && !FWD && p.skip_factor_one && *p.grad == 1.f) return;  // the forward has written this gradient
   const int V = (int)p.V, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float c = p.inv_temperature * kLog2e;
+  Stream<T, VEC, FWD && GRAD ? 2 : 1> stream(p, ring);
+  Pack<T, VEC> raw[kUnit];
   float count_inv = GRAD && !FWD && p.count ? 1.f / fmaxf(*p.count, 1.f) : 1.f;
   bool counted = false;
   for (long long row = blockIdx.x; row < p.N; row += gridDim.x) {
     const Row<T, VEC> r(static_cast<const T*>(p.logits) + row * p.ld, V);
-    const T* body = r.z + r.head;
     // the row's kept entries come in while the logits are read
     Entry e[2];
 #pragma unroll
@@ -106,22 +161,13 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
     if (FWD) {
       m = kNegInf;
       s = 0.f;
-      for (unsigned v0 = threadIdx.x; v0 < r.vectors; v0 += kUnroll * blockDim.x) {
-        Pack<T, VEC> raw[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-          if (v0 + u * blockDim.x < r.vectors) raw[u] = *reinterpret_cast<const Pack<T, VEC>*>(body + (size_t)(v0 + u * blockDim.x) * VEC);
+      unsigned v0 = threadIdx.x;
+      do {
+        stream.take(raw);
         float top = m;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          if (v0 + u * blockDim.x < r.vectors) {
-#pragma unroll
-            for (int k = 0; k < VEC / 2; ++k) {
-              const float2 x = pair_of(raw[u], k);
-              top = fmaxf(top, fmaxf(x.x, x.y));
-            }
-          }
-        }
+        for (int u = 0; u < kUnit; ++u)
+          if (v0 + u * blockDim.x < r.vectors) top = fmaxf(top, max_of(raw[u]));
         if (top > m) {
           s *= exp2_fast((m - top) * c);
           m = top;
@@ -129,7 +175,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
         const float2 minus = both(-finite_max(m));
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
+        for (int u = 0; u < kUnit; ++u) {
           if (v0 + u * blockDim.x < r.vectors) {
 #pragma unroll
             for (int k = 0; k < VEC / 2; ++k) {
@@ -139,7 +185,8 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
           }
         }
         s += sum.x + sum.y;
-      }
+        v0 += kUnit * blockDim.x;
+      } while (v0 - threadIdx.x < r.vectors);
       for (int g = threadIdx.x; g < r.head + r.tail; g += blockDim.x) {
         const float x = to_f32<T>(r.z[r.ragged(g, V)]);
         if (x > m) {
@@ -215,31 +262,24 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
       T* d_body = d + r.head;
       const float factor = any ? (FWD ? 1.f : p.grad[p.grad_per_row ? row * p.grad_ld : 0]) * count_inv * p.temperature : 0.f;
       const float scale = any ? factor / s : 0.f;
-      if (any) {
-        const float2 minus = both(-m);
-        for (unsigned v0 = threadIdx.x; v0 < r.vectors; v0 += kUnroll * blockDim.x) {
-          Pack<T, VEC> raw[kUnroll];
+      const float2 minus = both(-m);
+      unsigned v0 = threadIdx.x;
+      do {
+        stream.take(raw);
 #pragma unroll
-          for (int u = 0; u < kUnroll; ++u)
-            if (v0 + u * blockDim.x < r.vectors) raw[u] = *reinterpret_cast<const Pack<T, VEC>*>(body + (size_t)(v0 + u * blockDim.x) * VEC);
+        for (int u = 0; u < kUnit; ++u) {
+          if (v0 + u * blockDim.x < r.vectors) {
 #pragma unroll
-          for (int u = 0; u < kUnroll; ++u) {
-            if (v0 + u * blockDim.x < r.vectors) {
-#pragma unroll
-              for (int k = 0; k < VEC / 2; ++k) {
-                const float2 x = mul2(add2(pair_of(raw[u], k), minus), both(c));
-                set_pair(raw[u], k, mul2(make_float2(exp2_fast(x.x), exp2_fast(x.y)), both(scale)));
-              }
-              *reinterpret_cast<Pack<T, VEC>*>(d_body + (size_t)(v0 + u * blockDim.x) * VEC) = raw[u];
+            for (int k = 0; k < VEC / 2; ++k) {
+              const float2 x = mul2(add2(pair_of(raw[u], k), minus), both(c));
+              const float2 q = mul2(make_float2(exp2_fast(x.x), exp2_fast(x.y)), both(scale));
+              set_pair(raw[u], k, any ? q : make_float2(0.f, 0.f));
             }
+            *reinterpret_cast<Pack<T, VEC>*>(d_body + (size_t)(v0 + u * blockDim.x) * VEC) = raw[u];
           }
         }
-      } else {
-        Pack<T, VEC> zero;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) zero.v[k] = from_f32<T>(0.f);
-        for (unsigned v = threadIdx.x; v < r.vectors; v += blockDim.x) *reinterpret_cast<Pack<T, VEC>*>(d_body + (size_t)v * VEC) = zero;
-      }
+        v0 += kUnit * blockDim.x;
+      } while (v0 - threadIdx.x < r.vectors);
       for (int g = threadIdx.x; g < r.head + r.tail; g += blockDim.x) {
         const int j = r.ragged(g, V);
         d[j] = from_f32<T>(any ? scale * exp2_fast((to_f32<T>(r.z[j]) - m) * c) : 0.f);
@@ -312,11 +352,11 @@ bool valid(const B200Distill* p) {
          (p->index_dtype == B200_I64 || p->index_dtype == B200_I32) && (!p->loss || p->ticket);
 }
 
-// Threads for a row: about two rounds of unrolled vectors, and at least half as many as there are kept entries.
+// Threads for a row: about two units, and at least half as many as there are kept entries.
 int row_threads(const B200Distill& p) {
   const long long vectors = p.V / (p.dtype == B200_F32 ? 4 : 8);
   int t = 32;
-  while (t < kMaxThreads && (vectors > 2LL * kUnroll * t || p.K > 2 * t)) t *= 2;
+  while (t < kMaxThreads && (vectors > 2LL * kUnit * t || p.K > 2 * t)) t *= 2;
   return t;
 }
 
@@ -334,11 +374,17 @@ int launch(const B200Distill& p, bool after, cudaStream_t s) {
   overlap.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &overlap;
   cfg.numAttrs = after ? 1 : 0;
-  cudaError_t e = cudaErrorInvalidValue;
-  if (p.dtype == B200_BF16) e = cudaLaunchKernelEx(&cfg, distill_kernel<__nv_bfloat16, 8, FWD, GRAD>, p);
-  else if (p.dtype == B200_F16) e = cudaLaunchKernelEx(&cfg, distill_kernel<__half, 8, FWD, GRAD>, p);
-  else if (p.dtype == B200_F32) e = cudaLaunchKernelEx(&cfg, distill_kernel<float, 4, FWD, GRAD>, p);
-  return (int)e;
+  cfg.dynamicSmemBytes = (size_t)kDepth * kUnit * 16 * threads;
+  auto start = [&](auto kernel) {
+    cudaError_t e = cudaSuccess;
+    if (cfg.dynamicSmemBytes > 32 * 1024)
+      e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDepth * kUnit * 16 * kMaxThreads);
+    return (int)(e == cudaSuccess ? cudaLaunchKernelEx(&cfg, kernel, p) : e);
+  };
+  if (p.dtype == B200_BF16) return start(distill_kernel<__nv_bfloat16, 8, FWD, GRAD>);
+  if (p.dtype == B200_F16) return start(distill_kernel<__half, 8, FWD, GRAD>);
+  if (p.dtype == B200_F32) return start(distill_kernel<float, 4, FWD, GRAD>);
+  return (int)cudaErrorInvalidValue;
 }
 
 }  // namespace

@@ -66,6 +66,39 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 template <typename T, int N>
 __device__ __forceinline__ float2 pair_of(const Pack<T, N>& p, int i) { return make_float2(to_f32<T>(p.v[2 * i]), to_f32<T>(p.v[2 * i + 1])); }
 template <int N>
+__device__ __forceinline__ float2 pair_of(const Pack<__nv_bfloat16, N>& p, int i) {  // the upper half of an fp32 number each
+  const unsigned w = reinterpret_cast<const unsigned*>(&p)[i];
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <int N>
+__device__ __forceinline__ float2 pair_of(const Pack<__half, N>& p, int i) { return __half22float2(reinterpret_cast<const __half2*>(&p)[i]); }
+// The largest element (one that is no number counts only if all are).
+template <int N>
+__device__ __forceinline__ float max_of(const Pack<float, N>& p) {
+  float m = p.v[0];
+#pragma unroll
+  for (int k = 1; k < N; ++k) m = fmaxf(m, p.v[k]);
+  return m;
+}
+template <typename T2, typename T, int N>
+__device__ __forceinline__ T2 max_pair(const Pack<T, N>& p) {
+  const T2* w = reinterpret_cast<const T2*>(&p);
+  T2 m = w[0];
+#pragma unroll
+  for (int k = 1; k < N / 2; ++k) m = __hmax2(m, w[k]);
+  return m;
+}
+template <int N>
+__device__ __forceinline__ float max_of(const Pack<__nv_bfloat16, N>& p) {
+  const __nv_bfloat162 m = max_pair<__nv_bfloat162>(p);
+  return fmaxf(__low2float(m), __high2float(m));
+}
+template <int N>
+__device__ __forceinline__ float max_of(const Pack<__half, N>& p) {
+  const __half2 m = max_pair<__half2>(p);
+  return fmaxf(__low2float(m), __high2float(m));
+}
+template <int N>
 __device__ __forceinline__ void set_pair(Pack<float, N>& p, int i, float2 v) { p.v[2 * i] = v.x; p.v[2 * i + 1] = v.y; }
 template <int N>
 __device__ __forceinline__ void set_pair(Pack<__nv_bfloat16, N>& p, int i, float2 v) {

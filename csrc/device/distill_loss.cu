@@ -19,8 +19,8 @@ using namespace rowvec;
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxThreads = 512;
-constexpr int kUnit = 4;   // vectors that a thread takes at a time: a unit of a row is kUnit vectors for each thread
-constexpr int kDepth = 3;  // units under way
+constexpr int kUnit = 2;   // vectors that a thread takes at a time: a unit of a row is kUnit vectors for each thread
+constexpr int kDepth = 4;  // units under way
 
 struct Shared {
   float2 student[kMaxThreads / 32], teacher[kMaxThreads / 32];  // each warp's (maximum, sum of exponentials)
@@ -31,15 +31,24 @@ struct Shared {
 };
 
 __device__ __forceinline__ float finite_max(float m) { return m == kNegInf ? 0.f : m; }
-// The pairs of 32 lanes, then of a block's warps, as one: (maximum, sum of the exponentials of c times the distance to it).
-__device__ __forceinline__ float2 join(float m, float s, float c) {
-  const float top = group_max(m, 32);
-  return make_float2(top, group_sum(s * exp2_fast((m - finite_max(top)) * c), 32));  // m = -inf: nothing, or a NaN
-}
-__device__ __forceinline__ float2 join_warps(const float2* sh, float c) {
-  const int lane = threadIdx.x & 31;
-  const float2 v = lane < blockDim.x / 32 ? sh[lane] : make_float2(kNegInf, 0.f);
-  return join(v.x, v.y, c);
+// (maximum, sum of the exponentials of c times the distance to it) of 32 lanes, for the student's logits and the teacher's at once: the
+// two chains of exchanges hide one another.
+__device__ __forceinline__ void join(float2& a, float2& b, float c) {
+  float ta = a.x, tb = b.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ta = fmaxf(ta, __shfl_xor_sync(0xffffffffu, ta, o));
+    tb = fmaxf(tb, __shfl_xor_sync(0xffffffffu, tb, o));
+  }
+  float sa = a.y * exp2_fast((a.x - finite_max(ta)) * c);  // maximum -inf: nothing, or a NaN
+  float sb = b.y * exp2_fast((b.x - finite_max(tb)) * c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sa += __shfl_xor_sync(0xffffffffu, sa, o);
+    sb += __shfl_xor_sync(0xffffffffu, sb, o);
+  }
+  a = make_float2(ta, sa);
+  b = make_float2(tb, sb);
 }
 
 __device__ __forceinline__ float teacher_at(const void* p, long long i, int dt) {
@@ -61,8 +70,22 @@ __device__ __forceinline__ bool present(const B200Distill& p, long long row, int
 struct Entry {
   int idx;      // -1: absent
   float value;  // the teacher's logit, then its share
-  float z;      // the student's logit
 };
+// The same as it stands in memory, asked for a row ahead.
+struct Asked {
+  long long index;
+  float value;
+};
+__device__ __forceinline__ void ask(const B200Distill& p, long long row, Asked (&a)[2]) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int k = threadIdx.x + q * blockDim.x;
+    if (k < p.K && row < p.N) {
+      a[q].index = index_at(p, row, k);
+      a[q].value = teacher_at(p.teacher, row * p.teacher_ld + k, p.teacher_dtype);
+    }
+  }
+}
 
 // A row: `head` elements up to the first 16-byte boundary, whole vectors, `tail` elements.
 template <typename T, int VEC>
@@ -90,6 +113,7 @@ struct Stream {
   int pass, put, got;
   unsigned at, vectors;
   const T* body;
+  const uint64_t keep = l2_evict_last(), drop = l2_evict_first();
   __device__ __forceinline__ Stream(const B200Distill& args, void* shared)
       : p(args), ring(static_cast<Pack<T, VEC>*>(shared) + threadIdx.x), row(blockIdx.x), pass(0), put(0), got(0), at(0) {
     enter();
@@ -107,7 +131,7 @@ struct Stream {
 #pragma unroll
       for (int u = 0; u < kUnit; ++u) {
         const unsigned v = at + u * blockDim.x + threadIdx.x;
-        if (v < vectors) copy16_async(ring + (put * kUnit + u) * blockDim.x, body + (size_t)v * VEC);
+        if (v < vectors) copy16_async(ring + (put * kUnit + u) * blockDim.x, body + (size_t)v * VEC, PASSES == 2 && pass == 0 ? keep : drop);
       }
       at += kUnit * blockDim.x;
       if (at >= vectors) {
@@ -142,21 +166,28 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
   Pack<T, VEC> raw[kUnit];
   float count_inv = GRAD && !FWD && p.count ? 1.f / fmaxf(*p.count, 1.f) : 1.f;
   bool counted = false;
+  Asked asked[2];
+  ask(p, blockIdx.x, asked);
   for (long long row = blockIdx.x; row < p.N; row += gridDim.x) {
     const Row<T, VEC> r(static_cast<const T*>(p.logits) + row * p.ld, V);
-    // the row's kept entries come in while the logits are read
     Entry e[2];
+    T z[2];  // the student's logits there, on their way while the row is read
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int k = threadIdx.x + q * blockDim.x;
       e[q].idx = -1;
-      if (k < p.K) {
-        const long long i = index_at(p, row, k);
-        e[q].value = teacher_at(p.teacher, row * p.teacher_ld + k, p.teacher_dtype);
-        if (i >= 0 && i < p.V) e[q].idx = (int)i;
-        else if (i >= p.V && p.bad_flag) *p.bad_flag = 1;
+      z[q] = from_f32<T>(0.f);
+      if (threadIdx.x + q * blockDim.x < p.K) {
+        const long long i = asked[q].index;
+        e[q].value = asked[q].value;
+        if (i >= 0 && i < p.V && e[q].value != kNegInf) {
+          e[q].idx = (int)i;
+          z[q] = r.z[i];
+        }
+        if (i >= p.V && p.bad_flag) *p.bad_flag = 1;
       }
     }
+    const int place = (int)threadIdx.x < r.head + r.tail ? r.ragged(threadIdx.x, V) : -1;  // at most 14 elements outside whole vectors
+    const T ragged = place >= 0 ? r.z[place] : from_f32<T>(0.f);
     float m, s;
     if (FWD) {
       m = kNegInf;
@@ -187,44 +218,44 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
         s += sum.x + sum.y;
         v0 += kUnit * blockDim.x;
       } while (v0 - threadIdx.x < r.vectors);
-      for (int g = threadIdx.x; g < r.head + r.tail; g += blockDim.x) {
-        const float x = to_f32<T>(r.z[r.ragged(g, V)]);
+      if (place >= 0) {
+        const float x = to_f32<T>(ragged);
         if (x > m) {
           s *= exp2_fast((m - x) * c);
           m = x;
         }
         s += exp2_fast((x - finite_max(m)) * c);
       }
-      const float2 mine = join(m, s, c);
-      if (lane == 0) sh.student[warp] = mine;
     } else {
       const float2 st = reinterpret_cast<const float2*>(p.stats)[row];
       m = st.x;
       s = st.y;
     }
-    // the teacher's softmax, in the same way
-    float t_top = kNegInf, t_sum = 0.f;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      if (e[q].idx >= 0 && e[q].value == kNegInf) e[q].idx = -1;
-      if (e[q].idx >= 0) {
-        t_top = fmaxf(t_top, e[q].value);
-        e[q].z = to_f32<T>(r.z[e[q].idx]);
-      }
-    }
+    // both softmax sums over the block
+    float2 t = make_float2(kNegInf, 0.f);
 #pragma unroll
     for (int q = 0; q < 2; ++q)
-      if (e[q].idx >= 0) t_sum += exp2_fast((e[q].value - finite_max(t_top)) * c);
-    const float2 kept = join(t_top, t_sum, c);
-    if (lane == 0) sh.teacher[warp] = kept;
+      if (e[q].idx >= 0) t.x = fmaxf(t.x, e[q].value);
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (e[q].idx >= 0) t.y += exp2_fast((e[q].value - finite_max(t.x)) * c);
+    float2 st = make_float2(m, s);
+    join(st, t, c);
+    if (lane == 0) {
+      sh.student[warp] = st;
+      sh.teacher[warp] = t;
+    }
     const bool any = __syncthreads_or(e[0].idx >= 0 || e[1].idx >= 0);
+    const bool mine = lane < blockDim.x / 32;
+    st = mine ? sh.student[lane] : make_float2(kNegInf, 0.f);
+    t = mine ? sh.teacher[lane] : make_float2(kNegInf, 0.f);
+    join(st, t, c);
     if (FWD) {
-      const float2 st = join_warps(sh.student, c);
       m = finite_max(st.x);
       s = st.y;
       if (p.stats && threadIdx.x == 0) reinterpret_cast<float2*>(p.stats)[row] = make_float2(m, s);
     }
-    const float2 t = join_warps(sh.teacher, c);
+    ask(p, row + gridDim.x, asked);
     const float t_log = logf(t.y), s_log = FWD ? logf(s) : 0.f;
     float part = 0.f;
 #pragma unroll
@@ -234,13 +265,14 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
       if (e[q].idx >= 0) {
         const float lp = (e[q].value - t.x) * p.inv_temperature - t_log;
         e[q].value = expf(lp);
-        if (FWD && e[q].value != 0.f) part += e[q].value * (lp - ((e[q].z - m) * p.inv_temperature - s_log));
+        if (FWD && e[q].value != 0.f) part += e[q].value * (lp - ((to_f32<T>(z[q]) - m) * p.inv_temperature - s_log));
       }
       if (GRAD) {
         sh.idx[k] = e[q].idx;
         sh.share[k] = e[q].value;
       }
     }
+    if (GRAD && threadIdx.x < 3 && p.K + threadIdx.x < B200_DISTILL_MAX_K) sh.idx[p.K + threadIdx.x] = -1;
     if (FWD) {
       part = group_sum(part, 32);
       if (lane == 0) sh.loss[warp] = part;
@@ -275,15 +307,12 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
               const float2 q = mul2(make_float2(exp2_fast(x.x), exp2_fast(x.y)), both(scale));
               set_pair(raw[u], k, any ? q : make_float2(0.f, 0.f));
             }
-            *reinterpret_cast<Pack<T, VEC>*>(d_body + (size_t)(v0 + u * blockDim.x) * VEC) = raw[u];
+            __stcs(reinterpret_cast<uint4*>(d_body + (size_t)(v0 + u * blockDim.x) * VEC), *reinterpret_cast<const uint4*>(&raw[u]));
           }
         }
         v0 += kUnit * blockDim.x;
       } while (v0 - threadIdx.x < r.vectors);
-      for (int g = threadIdx.x; g < r.head + r.tail; g += blockDim.x) {
-        const int j = r.ragged(g, V);
-        d[j] = from_f32<T>(any ? scale * exp2_fast((to_f32<T>(r.z[j]) - m) * c) : 0.f);
-      }
+      if (place >= 0) d[place] = from_f32<T>(any ? scale * exp2_fast((to_f32<T>(ragged) - m) * c) : 0.f);
       __syncthreads();
       // the kept entries: the first occurrence of an index writes the value with the shares of all of them
 #pragma unroll
@@ -292,12 +321,18 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
         if (i < 0) continue;
         bool first = true;
         float share = 0.f;
-        for (int o = 0; o < p.K; ++o) {
-          if (sh.idx[o] != i) continue;
-          first = first && o >= k;
-          share += sh.share[o];
+        for (int o = 0; o < p.K; o += 4) {  // (behind the last entry: -1)
+          const int4 at = *reinterpret_cast<const int4*>(sh.idx + o);
+          if (at.x != i && at.y != i && at.z != i && at.w != i) continue;
+          const int four[4] = {at.x, at.y, at.z, at.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (four[u] != i) continue;
+            first = first && o + u >= k;
+            share += sh.share[o + u];
+          }
         }
-        if (first) d[i] = from_f32<T>(scale * exp2_fast((e[q].z - m) * c) - factor * share);
+        if (first) d[i] = from_f32<T>(scale * exp2_fast((to_f32<T>(z[q]) - m) * c) - factor * share);
       }
     }
   }
@@ -352,11 +387,13 @@ bool valid(const B200Distill* p) {
          (p->index_dtype == B200_I64 || p->index_dtype == B200_I32) && (!p->loss || p->ticket);
 }
 
-// Threads for a row: about two units, and at least half as many as there are kept entries.
+// Threads for a row: 30 vectors for each, and at least half as many as there are kept entries.  Small blocks because a row's
+// reductions leave an SM idle unless others are at work (4096 x 30522 bf16 with gradient: 164 us in blocks of 512, 129 in blocks of 128);
+// not smaller, because more rows in work do not stay in L2 until their second pass (4096 x 131072: 534 us with 512, 603 with 256).
 int row_threads(const B200Distill& p) {
   const long long vectors = p.V / (p.dtype == B200_F32 ? 4 : 8);
   int t = 32;
-  while (t < kMaxThreads && (vectors > 2LL * kUnit * t || p.K > 2 * t)) t *= 2;
+  while (t < kMaxThreads && (vectors > 30LL * t || p.K > 2 * t)) t *= 2;
   return t;
 }
 

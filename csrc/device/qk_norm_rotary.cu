@@ -63,31 +63,112 @@ __device__ __forceinline__ void place(int unit, int R, int& lo, int& hi, bool& r
   else { lo = unit * VEC; hi = R / 2 + unit * VEC; rot = true; }
 }
 
+// The arithmetic takes elements in pairs, two to an instruction, wherever a vector has any.
+template <int VEC>
+__device__ __forceinline__ float2 pair(const float (&a)[VEC], int i) { return make_float2(a[2 * i], a[2 * i + 1]); }
+template <int VEC>
+__device__ __forceinline__ void put(float (&a)[VEC], int i, float2 v) {
+  a[2 * i] = v.x;
+  a[2 * i + 1] = v.y;
+}
+// a = a * b
+template <int VEC>
+__device__ __forceinline__ void times(float (&a)[VEC], const float (&b)[VEC]) {
+  if constexpr (VEC == 1) a[0] *= b[0];
+  else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) put(a, i, mul2(pair(a, i), pair(b, i)));
+  }
+}
+// acc += a * b, element by element
+template <int VEC>
+__device__ __forceinline__ void add_products(float (&acc)[VEC], const float (&a)[VEC], const float (&b)[VEC]) {
+  if constexpr (VEC == 1) acc[0] = fmaf(a[0], b[0], acc[0]);
+  else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) put(acc, i, fma2(pair(a, i), pair(b, i), pair(acc, i)));
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void scale(float (&a)[VEC], float f) {
+  float v[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) v[k] = f;
+  times(a, v);
+}
+template <int VEC>
+__device__ __forceinline__ float total(const float (&a)[VEC]) {
+  float t = a[0];
+#pragma unroll
+  for (int k = 1; k < VEC; ++k) t += a[k];
+  return t;
+}
+
 template <int VEC, bool INTER>
 __device__ __forceinline__ void turn(float (&a)[VEC], float (&b)[VEC], const float (&c)[VEC], const float (&s)[VEC]) {
-  if (!INTER) {
+  if constexpr (VEC == 1) {
+    const float x = a[0], y = b[0];
+    a[0] = x * c[0] - y * s[0];
+    b[0] = y * c[0] + x * s[0];
+  } else if constexpr (!INTER) {
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      const float x = a[k], y = b[k];
-      a[k] = x * c[k] - y * s[k];
-      b[k] = y * c[k] + x * s[k];
+    for (int i = 0; i < VEC / 2; ++i) {
+      const float2 x = pair(a, i), y = pair(b, i), cc = pair(c, i), ss = pair(s, i);
+      put(a, i, fma2(y, make_float2(-ss.x, -ss.y), mul2(x, cc)));
+      put(b, i, fma2(x, ss, mul2(y, cc)));
     }
   } else {
     // the unit is one run of 2 VEC elements: pair i is (2i, 2i + 1)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      float& x = 2 * i < VEC ? a[(2 * i) % VEC] : b[(2 * i) % VEC];
-      float& y = 2 * i + 1 < VEC ? a[(2 * i + 1) % VEC] : b[(2 * i + 1) % VEC];
-      const float u = x, v = y;
-      x = u * c[i] - v * s[i];
-      y = v * c[i] + u * s[i];
+      float(&v)[VEC] = 2 * i < VEC ? a : b;
+      const int k = i % (VEC / 2);
+      const float2 x = pair(v, k);
+      put(v, k, fma2(make_float2(x.y, x.x), make_float2(-s[i], s[i]), mul2(x, both(c[i]))));
     }
   }
 }
 
+// A group's way through its heads: item after item, the heads of an item in turn.
+struct Cursor {
+  unsigned item, token;
+  int i, h0, hn;            // head within the item; the item's first head and number of heads (0: no item)
+  long long x_at, g_at;     // the token's place
+  unsigned b, l;
+  __device__ __forceinline__ void enter(const Args& p, const Side& sd, unsigned at) {
+    item = at;
+    i = 0;
+    hn = 0;
+    token = b = l = 0;
+    h0 = 0;
+    if (at < sd.items) {
+      token = at / (unsigned)sd.items_per_token;
+      h0 = (int)(at % (unsigned)sd.items_per_token) * sd.heads_per_item;
+      hn = min(sd.heads_per_item, sd.heads - h0);
+      b = token / p.L;
+      l = token % p.L;
+    }
+    x_at = b * sd.xs_b + l * sd.xs_l;
+    g_at = b * sd.gs_b + l * sd.gs_l;
+  }
+  // returns whether a new item has begun
+  __device__ __forceinline__ bool advance(const Args& p, const Side& sd, unsigned stride) {
+    if (++i < sd.heads_per_item) return false;
+    enter(p, sd, item < sd.items ? item + stride : item);
+    return true;
+  }
+};
+
+constexpr int ring_depth(bool bwd) { return bwd ? 3 : 4; }
+constexpr int resident_blocks(int ch, bool bwd) { return ch > 1 ? 1 : (bwd ? 2 : 3); }
+
 template <typename T, int VEC, int CH, bool INTER, bool BWD>
-__global__ void __launch_bounds__(kThreads) qk_norm_rotary_kernel(const __grid_constant__ Args p) {
-  extern __shared__ float sh_dw[];  // backward: [warps][D]
+__global__ void __launch_bounds__(kThreads, resident_blocks(CH, BWD)) qk_norm_rotary_kernel(const __grid_constant__ Args p) {
+  // heads on their way: each thread copies its vectors of the next heads to a place of its own.  Behind the last head: partial dw.
+  extern __shared__ __align__(16) unsigned char shared[];
+  using V = Pack<T, VEC>;
+  constexpr bool kAsync = sizeof(V) >= 4;
+  constexpr int kDepth = ring_depth(BWD), kPerHead = CH * 2 * (BWD ? 2 : 1);
   const bool keys = blockIdx.x >= (unsigned)p.side[0].blocks;
   const Side& sd = p.side[keys ? 1 : 0];
   const unsigned block = keys ? blockIdx.x - p.side[0].blocks : blockIdx.x;
@@ -102,13 +183,47 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rotary_kernel(const __grid_c
 
   int lo[CH], hi[CH];
   bool rot[CH], on[CH];
-  float wl[CH][VEC], wh[CH][VEC];
-  float dl[CH][VEC], dh[CH][VEC];  // backward: this lane's part of dw
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int u = gl + c * G;
     on[c] = u < units;
     place<VEC, INTER>(on[c] ? u : 0, p.R, lo[c], hi[c], rot[c]);
+  }
+
+  // All groups of a warp run the same number of rounds, since the reductions take the whole warp.
+  const unsigned stride = (unsigned)sd.blocks * groups_per_block;
+  const unsigned first = block * groups_per_block + threadIdx.x / G;
+  const unsigned warp_first = block * groups_per_block + (threadIdx.x & ~31u) / G;
+  V* ring = reinterpret_cast<V*>(shared) + threadIdx.x;
+  Cursor ahead;
+  ahead.enter(p, sd, first);
+  auto fetch = [&](int stage) {
+    if (kAsync) {
+      const bool there = ahead.i < ahead.hn;
+      const int h = ahead.h0 + (there ? ahead.i : 0);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        V* slot = ring + (stage * kPerHead + c * (BWD ? 4 : 2)) * kThreads;
+        const T* xh = x + ahead.x_at + h * sd.xs_h;
+        copy_async<kAsync ? sizeof(V) : 4>(slot, xh + lo[c], there && on[c]);
+        copy_async<kAsync ? sizeof(V) : 4>(slot + kThreads, xh + hi[c], there && on[c]);
+        if (BWD) {
+          const T* gh = dy + ahead.g_at + h * sd.gs_h;
+          copy_async<kAsync ? sizeof(V) : 4>(slot + 2 * kThreads, gh + lo[c], there && on[c]);
+          copy_async<kAsync ? sizeof(V) : 4>(slot + 3 * kThreads, gh + hi[c], there && on[c]);
+        }
+      }
+      ahead.advance(p, sd, stride);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int d = 0; d < kDepth - 1; ++d) fetch(d);
+
+  float wl[CH][VEC], wh[CH][VEC];
+  float dl[CH][VEC], dh[CH][VEC];  // backward: this lane's part of dw
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
       wl[c][k] = sd.weight ? weight_at(sd.weight, sd.weight_dtype, lo[c] + k) : 1.f;
@@ -117,28 +232,23 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rotary_kernel(const __grid_c
     }
   }
 
-  // All groups of a warp run the same number of rounds, since the reductions take the whole warp.
-  const unsigned stride = (unsigned)sd.blocks * groups_per_block;
-  const unsigned first = block * groups_per_block + threadIdx.x / G;
-  const unsigned warp_first = block * groups_per_block + (threadIdx.x & ~31u) / G;
+  Cursor now;
+  int stage = 0;
   for (unsigned long long base = warp_first, item = first; base < sd.items; base += stride, item += stride) {
-    const bool live = item < sd.items;
-    const unsigned token = live ? (unsigned)item / (unsigned)sd.items_per_token : 0;
-    const unsigned part = live ? (unsigned)item % (unsigned)sd.items_per_token : 0;
-    const unsigned b = token / p.L, l = token % p.L;
-    long long pos = l;
+    now.enter(p, sd, item < sd.items ? (unsigned)item : sd.items);
+    long long pos = now.l;
     if (p.positions) {
-      const long long at = b * p.pos_b + l * p.pos_l;
+      const long long at = now.b * p.pos_b + now.l * p.pos_l;
       pos = p.pos_is_64 ? static_cast<const long long*>(p.positions)[at] : (long long)static_cast<const int*>(p.positions)[at];
     }
-    const bool inside = pos >= 0 && pos < p.table_rows;
-    if (live && !inside && p.bad_flag && gl == 0) *p.bad_flag = 1;
+    const bool inside = now.hn > 0 && pos >= 0 && pos < p.table_rows;
+    if (now.hn > 0 && !inside && p.bad_flag && gl == 0) *p.bad_flag = 1;
     float cs[CH][VEC], sn[CH][VEC];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) { cs[c][k] = 1.f; sn[c][k] = 0.f; }
-      if (live && inside && on[c] && rot[c]) {
+      if (inside && on[c] && rot[c]) {
         const long long at = pos * (p.R / 2) + (INTER ? lo[c] / 2 : lo[c]);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
@@ -147,74 +257,88 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rotary_kernel(const __grid_c
         }
       }
     }
-    const int h0 = (int)part * sd.heads_per_item;
-    const int hn = live ? min(sd.heads_per_item, sd.heads - h0) : 0;
-    const T* xt = x + b * sd.xs_b + l * sd.xs_l;
-    const T* gt = BWD ? dy + b * sd.gs_b + l * sd.gs_l : nullptr;
-    T* ot = out + (long long)token * sd.heads * p.D;
-    for (int i = 0; i < sd.heads_per_item; ++i) {
-      const bool act = i < hn;
-      const int h = h0 + (act ? i : 0);
-      float a[CH][VEC], z[CH][VEC];
-      float ss = 0.f;
+    T* ot = out + ((long long)now.token * sd.heads + now.h0) * p.D;
+    for (int i = 0; i < sd.heads_per_item; ++i, ot += p.D) {
+      const bool act = i < now.hn;
+      fetch(stage == 0 ? kDepth - 1 : stage - 1);
+      copies_wait<kDepth - 1>();
+      V raw[CH][BWD ? 4 : 2];
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) a[c][k] = z[c][k] = 0.f;
-        if (act && on[c]) {
-          load<T, VEC>(xt + h * sd.xs_h + lo[c], a[c]);
-          load<T, VEC>(xt + h * sd.xs_h + hi[c], z[c]);
-        }
+        for (int n = 0; n < (BWD ? 4 : 2); ++n) {
+          if (kAsync) {
+            raw[c][n] = ring[(stage * kPerHead + c * (BWD ? 4 : 2) + n) * kThreads];
+          } else {
+            const T* from = n < 2 ? x + now.x_at + (now.h0 + i) * sd.xs_h : dy + now.g_at + (now.h0 + i) * sd.gs_h;
+            if (act && on[c]) raw[c][n] = *reinterpret_cast<const V*>(from + (n % 2 ? hi[c] : lo[c]));
+          }
+          if (!inside || (!kAsync && !(act && on[c]))) {  // what a token outside the tables holds counts for nothing
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) ss += a[c][k] * a[c][k] + z[c][k] * z[c][k];
+            for (int k = 0; k < VEC; ++k) raw[c][n].v[k] = from_f32<T>(0.f);
+          }
+        }
+      }
+      stage = stage == kDepth - 1 ? 0 : stage + 1;
+      float a[CH][VEC], z[CH][VEC], sq[VEC], dt[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sq[k] = dt[k] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        unpack(raw[c][0], a[c]);
+        unpack(raw[c][1], z[c]);
+        add_products(sq, a[c], a[c]);
+        add_products(sq, z[c], z[c]);
       }
       if (!BWD) {
-        const float r = rsqrtf(group_sum(ss, G) * inv_d + p.eps);
+        const float r = rsqrtf(group_sum(total(sq), G) * inv_d + p.eps);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) {
-            a[c][k] = inside ? a[c][k] * (r * wl[c][k]) : 0.f;
-            z[c][k] = inside ? z[c][k] * (r * wh[c][k]) : 0.f;
-          }
+          scale(a[c], inside ? r : 0.f);
+          scale(z[c], inside ? r : 0.f);
+          times(a[c], wl[c]);
+          times(z[c], wh[c]);
           turn<VEC, INTER>(a[c], z[c], cs[c], sn[c]);
           if (act && on[c]) {
-            store<T, VEC>(ot + (long long)h * p.D + lo[c], a[c]);
-            store<T, VEC>(ot + (long long)h * p.D + hi[c], z[c]);
+            store<T, VEC>(ot + lo[c], a[c]);
+            store<T, VEC>(ot + hi[c], z[c]);
           }
         }
       } else {
         float ga[CH][VEC], gz[CH][VEC];
-        float dot = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) ga[c][k] = gz[c][k] = 0.f;
-          if (act && on[c] && inside) {
-            load<T, VEC>(gt + h * sd.gs_h + lo[c], ga[c]);
-            load<T, VEC>(gt + h * sd.gs_h + hi[c], gz[c]);
-          }
+          unpack(raw[c][2], ga[c]);
+          unpack(raw[c][3], gz[c]);
           turn<VEC, INTER>(ga[c], gz[c], cs[c], sn[c]);
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) dot += ga[c][k] * wl[c][k] * a[c][k] + gz[c][k] * wh[c][k] * z[c][k];
         }
-        const float r = rsqrtf(group_sum(ss, G) * inv_d + p.eps);
-        const float m = group_sum(dot, G) * inv_d * r * r;
+        float ss = total(sq);
+        for (int o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float r = act && inside ? rsqrtf(ss * inv_d + p.eps) : 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          float da[VEC], dz[VEC];
+          scale(a[c], r);  // the normalised head
+          scale(z[c], r);
+          add_products(dl[c], ga[c], a[c]);
+          add_products(dh[c], gz[c], z[c]);
+          times(ga[c], wl[c]);
+          times(gz[c], wh[c]);
+          add_products(dt, ga[c], a[c]);
+          add_products(dt, gz[c], z[c]);
+        }
+        const float m = -group_sum(total(dt), G) * inv_d;
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) {
-            if (act && inside) {
-              dl[c][k] += ga[c][k] * a[c][k] * r;
-              dh[c][k] += gz[c][k] * z[c][k] * r;
-            }
-            da[k] = inside ? r * (ga[c][k] * wl[c][k] - a[c][k] * m) : 0.f;
-            dz[k] = inside ? r * (gz[c][k] * wh[c][k] - z[c][k] * m) : 0.f;
-          }
+        for (int c = 0; c < CH; ++c) {
+          float v[VEC];
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) v[k] = m;
+          add_products(ga[c], a[c], v);
+          add_products(gz[c], z[c], v);
+          scale(ga[c], r);
+          scale(gz[c], r);
           if (act && on[c]) {
-            store<T, VEC>(ot + (long long)h * p.D + lo[c], da);
-            store<T, VEC>(ot + (long long)h * p.D + hi[c], dz);
+            store<T, VEC>(ot + lo[c], ga[c]);
+            store<T, VEC>(ot + hi[c], gz[c]);
           }
         }
       }
@@ -223,6 +347,9 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rotary_kernel(const __grid_c
 
   if (BWD && sd.dw_partial) {
     // the groups of a warp, then the warps, in a fixed order: the same inputs give the same bits
+    copies_wait<0>();
+    __syncthreads();
+    float* sh_dw = reinterpret_cast<float*>(shared);  // [warps][D]
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
 #pragma unroll
@@ -310,45 +437,56 @@ Plan make_plan(const B200QkNormRotary& p, bool bwd) {
   a.cos = p.cos; a.sin = p.sin; a.positions = p.positions; a.pos_b = p.pos_stride[0]; a.pos_l = p.pos_stride[1];
   a.pos_is_64 = p.positions_dtype == B200_I64; a.table_rows = p.table_rows; a.bad_flag = p.bad_flag;
   a.L = (unsigned)p.L; a.D = p.D; a.R = p.R; a.eps = p.eps;
-  const long long tokens = p.B * p.L;
+  const long long tokens = p.B * p.L, heads = (long long)p.side[0].heads + p.side[1].heads;
+  // Heads per item, which share a token's cos / sin and place: as many as leave every SM 512 threads, at most eight.
+  int hpi = 1;
+  while (hpi < 8 && tokens * heads / (hpi * 2) * a.group >= 148LL * 512) hpi *= 2;
+  const long long per_block = kThreads / a.group, resident = 148 * resident_blocks(pl.ch, bwd);
   for (int s = 0; s < 2; ++s) {
     const B200QkSide& q = p.side[s];
     Side& d = a.side[s];
     d.x = q.x; d.dy = q.dy; d.out = q.out; d.weight = q.weight; d.weight_dtype = q.weight_dtype; d.heads = q.heads;
     d.xs_b = q.x_stride[0]; d.xs_l = q.x_stride[1]; d.xs_h = q.x_stride[2];
     d.gs_b = q.dy_stride[0]; d.gs_l = q.dy_stride[1]; d.gs_h = q.dy_stride[2];
-    // heads per item: as many as keep every SM busy with about 1024 threads, at most eight
-    int hpi = 1;
-    while (hpi < 8 && hpi * 2 <= q.heads && tokens * (q.heads / (hpi * 2)) * a.group >= 148LL * 1024) hpi *= 2;
-    d.heads_per_item = hpi;
-    d.items_per_token = (q.heads + hpi - 1) / hpi;
+    if (q.heads == 0) continue;
+    d.heads_per_item = hpi < q.heads ? hpi : q.heads;
+    d.items_per_token = (q.heads + d.heads_per_item - 1) / d.heads_per_item;
     d.items = (unsigned)(tokens * d.items_per_token);
-    const long long per_block = kThreads / a.group;
-    long long blocks = (d.items + per_block - 1) / per_block;
-    const long long most = bwd ? 148 * 4 : 148 * 64;
-    d.blocks = (int)(blocks < most ? blocks : most);
+    // one wave of blocks, shared out by the number of heads
+    const long long blocks = (d.items + per_block - 1) / per_block, share = (resident * q.heads + heads - 1) / heads;
+    d.blocks = (int)(blocks < share ? blocks : share);
     pl.grid += d.blocks;
   }
   return pl;
 }
 
+template <typename T, int VEC, int CH, bool INTER, bool BWD>
+int launch_one(const Plan& pl, cudaStream_t s) {
+  size_t smem = (size_t)ring_depth(BWD) * CH * 2 * (BWD ? 2 : 1) * kThreads * sizeof(T) * VEC;
+  const size_t dw = BWD ? (size_t)(kThreads / 32) * pl.a.D * sizeof(float) : 0;
+  if (smem < dw) smem = dw;
+  auto kernel = qk_norm_rotary_kernel<T, VEC, CH, INTER, BWD>;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+  }
+  kernel<<<pl.grid, kThreads, smem, s>>>(pl.a);
+  return (int)cudaGetLastError();
+}
 template <typename T, int VEC, int CH, bool BWD>
-void launch(const Plan& pl, bool interleaved, cudaStream_t s) {
-  const size_t smem = BWD ? (size_t)(kThreads / 32) * pl.a.D * sizeof(float) : 0;
-  if (interleaved) qk_norm_rotary_kernel<T, VEC, CH, true, BWD><<<pl.grid, kThreads, smem, s>>>(pl.a);
-  else qk_norm_rotary_kernel<T, VEC, CH, false, BWD><<<pl.grid, kThreads, smem, s>>>(pl.a);
+int launch(const Plan& pl, bool interleaved, cudaStream_t s) {
+  return interleaved ? launch_one<T, VEC, CH, true, BWD>(pl, s) : launch_one<T, VEC, CH, false, BWD>(pl, s);
 }
 template <typename T, int WIDEST, bool BWD>
 int dispatch(const Plan& pl, bool interleaved, cudaStream_t s) {
   // units of one head: D / (2 VEC) over at most 32 lanes, D at most 512
-  if (pl.vec == 8 && WIDEST == 8) launch<T, WIDEST == 8 ? 8 : 4, 1, BWD>(pl, interleaved, s);
-  else if (pl.vec == 4 && pl.ch == 1) launch<T, 4, 1, BWD>(pl, interleaved, s);
-  else if (pl.vec == 4) launch<T, 4, 2, BWD>(pl, interleaved, s);
-  else if (pl.vec == 2 && pl.ch == 1) launch<T, 2, 1, BWD>(pl, interleaved, s);
-  else if (pl.vec == 2) launch<T, 2, 4, BWD>(pl, interleaved, s);
-  else if (pl.ch == 1) launch<T, 1, 1, BWD>(pl, interleaved, s);
-  else launch<T, 1, 8, BWD>(pl, interleaved, s);
-  return (int)cudaGetLastError();
+  if (pl.vec == 8 && WIDEST == 8) return launch<T, WIDEST == 8 ? 8 : 4, 1, BWD>(pl, interleaved, s);
+  if (pl.vec == 4 && pl.ch == 1) return launch<T, 4, 1, BWD>(pl, interleaved, s);
+  if (pl.vec == 4) return launch<T, 4, 2, BWD>(pl, interleaved, s);
+  if (pl.vec == 2 && pl.ch == 1) return launch<T, 2, 1, BWD>(pl, interleaved, s);
+  if (pl.vec == 2) return launch<T, 2, 4, BWD>(pl, interleaved, s);
+  if (pl.ch == 1) return launch<T, 1, 1, BWD>(pl, interleaved, s);
+  return launch<T, 1, 8, BWD>(pl, interleaved, s);
 }
 
 bool valid(const B200QkNormRotary* p) {

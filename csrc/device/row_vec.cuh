@@ -23,6 +23,17 @@ template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
 __device__ __forceinline__ void copy16_async(void* shared, const void* global) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(shared)), "l"(global) : "memory");
 }
+// 4, 8 or 16 bytes, or zeros in their place.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* shared, const void* global, bool there) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(shared)), "l"(global), "r"(there ? 16 : 0)
+                 : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"((unsigned)__cvta_generic_to_shared(shared)), "l"(global), "n"(BYTES),
+                 "r"(there ? BYTES : 0)
+                 : "memory");
+}
 // The same with a policy for L2.
 __device__ __forceinline__ void copy16_async(void* shared, const void* global, uint64_t policy) {
   asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(shared)), "l"(global), "l"(policy)
@@ -87,6 +98,18 @@ __device__ __forceinline__ float2 pair_of(const Pack<__nv_bfloat16, N>& p, int i
 }
 template <int N>
 __device__ __forceinline__ float2 pair_of(const Pack<__half, N>& p, int i) { return __half22float2(reinterpret_cast<const __half2*>(&p)[i]); }
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const Pack<T, N>& p, float (&out)[N]) {
+  if constexpr (N == 1) out[0] = to_f32<T>(p.v[0]);
+  else {
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+      const float2 v = pair_of(p, k);
+      out[2 * k] = v.x;
+      out[2 * k + 1] = v.y;
+    }
+  }
+}
 // The largest element (one that is no number counts only if all are).
 template <int N>
 __device__ __forceinline__ float max_of(const Pack<float, N>& p) {

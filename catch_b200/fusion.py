@@ -413,7 +413,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     chooses the rows of the tables, by default ``0 .. length - 1``; a token whose position lies outside them (a padding token
     marked with -1) gives zeros and gets zero gradients.  The results are contiguous and have the inputs' dtype; sums are taken in
     fp32.  Differentiable in ``q``, ``k`` and the weights."""
-    return torch.ops.catch_b200.qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    return torch.ops.catch_b200.qk_norm_rotary.default(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
 
 def relative_bias_softmax(scores: torch.Tensor, table: torch.Tensor, mask: Optional[torch.Tensor] = None, *, scale: float = 1.0,
@@ -426,7 +426,7 @@ def relative_bias_softmax(scores: torch.Tensor, table: torch.Tensor, mask: Optio
     farther ones share the rest by logarithm, and all from ``max_distance`` on share the last.  ``mask`` broadcasts to the
     scores: bool (``True`` keeps a key) or floating (added; ``-inf`` excludes a key whatever its score holds).  A row without any key left
     gives zeros.  Differentiable in ``scores`` and ``table``; the bias is never stored as a matrix."""
-    return torch.ops.catch_b200.relative_bias_softmax(scores, table, mask, scale, bidirectional, max_distance, query_offset)[0]
+    return torch.ops.catch_b200.relative_bias_softmax.default(scores, table, mask, scale, bidirectional, max_distance, query_offset)[0]
 
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -443,7 +443,7 @@ def top_logits_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, 
     ``"mean"`` over the rows that count, ``"sum"`` or ``"none"``; the loss is fp32.  Differentiable in ``logits``."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"top_logits_distillation: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
-    return torch.ops.catch_b200.top_logits_distillation(logits, teacher_logits, teacher_index, temperature, _REDUCTIONS[reduction])
+    return torch.ops.catch_b200.top_logits_distillation.default(logits, teacher_logits, teacher_index, temperature, _REDUCTIONS[reduction])
 
 
 def _feeds_only(node: fx.Node, consumer: fx.Node) -> bool:

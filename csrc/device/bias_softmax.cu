@@ -678,8 +678,14 @@ __global__ void __launch_bounds__(kMaxThreads) bias_table_grad(const float* part
   float t = 0.f;
   if (lo <= hi) {
     const float* mine = partial + (long long)h * blocks * slots + x0;
-    const unsigned run = (unsigned)(x1 - x0 + 1), n = run * (unsigned)blocks;
-    for (unsigned i = threadIdx.x; i < n; i += blockDim.x) t += mine[(long long)(i / run) * slots + i % run];
+    const int run = x1 - x0 + 1, wide = run < (int)blockDim.x ? run : (int)blockDim.x, rows = blockDim.x / wide;
+    const int x = threadIdx.x % wide, row = threadIdx.x / wide;
+    if (row < rows) {
+      for (int i = x; i < run; i += wide) {
+#pragma unroll 8
+        for (int b = row; b < blocks; b += rows) t += mine[(long long)b * slots + i];
+      }
+    }
   }
   t = block_sum(t, sh);
   if (threadIdx.x == 0) {

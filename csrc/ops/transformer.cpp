@@ -7,8 +7,10 @@
 // calls).  Every operator has a host path in elementary operations for host simulation and for tensors of other
 // devices; gradients are wired up here, so torch.ops.catch_b200.<name> is differentiable as it is.
 #include <ATen/core/grad_mode.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -25,7 +27,7 @@ namespace ops {
 namespace {
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 using OptTensor = std::optional<Tensor>;
 
@@ -33,7 +35,10 @@ constexpr double kInf = std::numeric_limits<double>::infinity();
 
 bool f_ok(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
-const void* ptr_or_null(const OptTensor& t) { return given(t) ? t->data_ptr() : nullptr; }
+// Uninitialised device tensors without a trip through the dispatcher.
+Tensor fresh(at::IntArrayRef sizes, const Tensor& like) { return empty_b200(sizes, like.scalar_type(), like.device().index()); }
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return empty_b200(sizes, type, like.device().index()); }
+Tensor fresh_strided(const Tensor& like) { return empty_strided_b200(like.sizes(), like.strides(), like.scalar_type(), like.device().index()); }
 bool on_device(const Tensor& t) { return !use_cpu_path() && is_b200(t); }
 
 // Results of a backward that is itself differentiated raise instead of counting as constants.
@@ -187,7 +192,7 @@ std::tuple<Tensor, Tensor> rotary_fwd(const RotaryArgs& a) {
   check_rotary(a);
   if (!on_device(a.q)) return {host_rotary_fwd(a, a.q, a.qw), host_rotary_fwd(a, a.k, a.kw)};
   OpScope scope("qk_norm_rotary", a.q);
-  Tensor q = dense_last(a.q), k = dense_last(a.k), yq = at::empty(q.sizes(), q.options()), yk = at::empty(k.sizes(), k.options());
+  Tensor q = dense_last(a.q), k = dense_last(a.k), yq = fresh(q.sizes(), q), yk = fresh(k.sizes(), k);
   const OptTensor qw = dense_weight(a.qw), kw = dense_weight(a.kw);
   std::vector<Tensor> keep;
   B200QkNormRotary p = rotary_params(a, q, k, qw, kw, keep);
@@ -198,7 +203,7 @@ std::tuple<Tensor, Tensor> rotary_fwd(const RotaryArgs& a) {
   return {yq, yk};
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> rotary_bwd(const RotaryArgs& a, const Tensor& dyq, const Tensor& dyk) {
+std::tuple<Tensor, Tensor, Tensor, Tensor> rotary_bwd(const RotaryArgs& a, const Tensor& dyq, const Tensor& dyk, bool need_qw = true, bool need_kw = true) {
   check_rotary(a);
   TORCH_CHECK(dyq.sizes() == a.q.sizes() && dyk.sizes() == a.k.sizes() && dyq.scalar_type() == a.q.scalar_type() &&
                   dyk.scalar_type() == a.k.scalar_type(),
@@ -211,10 +216,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rotary_bwd(const RotaryArgs& a, const
   }
   OpScope scope("qk_norm_rotary_backward", a.q);
   Tensor q = dense_last(a.q), k = dense_last(a.k), gq = dense_last(dyq), gk = dense_last(dyk);
-  Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dqw, dkw;
+  Tensor dq = fresh(q.sizes(), q), dk = fresh(k.sizes(), k), dqw, dkw;
   const OptTensor qw = dense_weight(a.qw), kw = dense_weight(a.kw);
-  if (given(qw)) dqw = at::empty_like(*qw);
-  if (given(kw)) dkw = at::empty_like(*kw);
+  if (given(qw) && need_qw) dqw = fresh(qw->sizes(), *qw);
+  if (given(kw) && need_kw) dkw = fresh(kw->sizes(), *kw);
   std::vector<Tensor> keep;
   B200QkNormRotary p = rotary_params(a, q, k, qw, kw, keep);
   const Tensor* g[2] = {&gq, &gk};
@@ -233,36 +238,51 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rotary_bwd(const RotaryArgs& a, const
 
 OptTensor saved_optional(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
+// ---- autograd.  Nodes of their own instead of torch::autograd::Function: the call of a small operator is as long as its bookkeeping.
 bool wants_grad(std::initializer_list<const Tensor*> leaves) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : leaves)
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+const Tensor& or_none(const OptTensor& t) {
+  static const Tensor none;
+  return given(t) ? *t : none;
+}
+template <typename N>
+std::shared_ptr<N> make_node() {
+  return std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
+}
+SavedVariable save(const Tensor& t) { return SavedVariable(t, /*is_output=*/false); }
+// Runs without recording, below autograd.
+struct Below {
+  at::AutoDispatchBelowADInplaceOrView dispatch;
+  at::NoGradGuard no_grad;
+};
 
-struct RotaryFn : public torch::autograd::Function<RotaryFn> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw,
-                               const Tensor& cos, const Tensor& sin, const OptTensor& positions, double eps, bool interleaved) {
-    at::AutoDispatchBelowADInplaceOrView guard;
-    ctx->save_for_backward({q, k, given(qw) ? *qw : Tensor(), given(kw) ? *kw : Tensor(), cos, sin, given(positions) ? *positions : Tensor()});
-    ctx->saved_data["eps"] = eps;
-    ctx->saved_data["interleaved"] = interleaved;
-    auto [yq, yk] = rotary_fwd({q, k, qw, kw, cos, sin, positions, eps, interleaved});
-    return {yq, yk};
+struct RotaryNode : public torch::autograd::Node {
+  SavedVariable q, k, qw, kw, cos, sin, positions;
+  double eps = 0;
+  bool interleaved = false;
+  std::string name() const override { return "QkNormRotaryBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* s : {&q, &k, &qw, &kw, &cos, &sin, &positions}) s->reset_data();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const variable_list s = ctx->get_saved_variables();
-    variable_list out(9);
+  variable_list apply(variable_list&& g) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(4);
+    if (!g[0].defined() && !g[1].defined()) return out;
+    const Tensor uq = q.unpack(), uk = k.unpack();
     {
-      at::AutoDispatchBelowADInplaceOrView guard;
-      at::NoGradGuard no_grad;
-      Tensor gq = g[0].defined() ? g[0] : at::zeros_like(s[0], at::MemoryFormat::Contiguous);
-      Tensor gk = g[1].defined() ? g[1] : at::zeros_like(s[1], at::MemoryFormat::Contiguous);
-      auto [dq, dk, dqw, dkw] = rotary_bwd({s[0], s[1], saved_optional(s[2]), saved_optional(s[3]), s[4], s[5], saved_optional(s[6]),
-                                            ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool()}, gq, gk);
-      out[0] = dq; out[1] = dk; out[2] = dqw; out[3] = dkw;
+      Below below;
+      Tensor gq = g[0].defined() ? g[0] : at::zeros_like(uq, at::MemoryFormat::Contiguous);
+      Tensor gk = g[1].defined() ? g[1] : at::zeros_like(uk, at::MemoryFormat::Contiguous);
+      std::tie(out[0], out[1], out[2], out[3]) =
+          rotary_bwd({uq, uk, saved_optional(qw.unpack()), saved_optional(kw.unpack()), cos.unpack(), sin.unpack(),
+                      saved_optional(positions.unpack()), eps, interleaved}, gq, gk, task_should_compute_output(2), task_should_compute_output(3));
     }
-    return once_differentiable("qk_norm_rotary", out);
+    return once_differentiable("qk_norm_rotary", std::move(out));
   }
 };
 
@@ -273,13 +293,26 @@ std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q, const Tensor& k, cons
 std::tuple<Tensor, Tensor> qk_norm_rotary_autograd(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw,
                                                    const Tensor& cos, const Tensor& sin, const OptTensor& positions, double eps,
                                                    bool interleaved) {
-  const Tensor none;
-  if (!wants_grad({&q, &k, given(qw) ? &*qw : &none, given(kw) ? &*kw : &none})) {
-    at::AutoDispatchBelowADInplaceOrView guard;
-    return qk_norm_rotary(q, k, qw, kw, cos, sin, positions, eps, interleaved);
+  std::shared_ptr<RotaryNode> node;
+  const Tensor &tqw = or_none(qw), &tkw = or_none(kw);
+  if (wants_grad({&q, &k, &tqw, &tkw})) {
+    node = make_node<RotaryNode>();
+    node->set_next_edges(torch::autograd::collect_next_edges(q, k, tqw, tkw));
+    node->q = save(q); node->k = save(k); node->qw = save(tqw); node->kw = save(tkw);
+    node->cos = save(cos); node->sin = save(sin); node->positions = save(or_none(positions));
+    node->eps = eps;
+    node->interleaved = interleaved;
   }
-  const variable_list y = RotaryFn::apply(q, k, qw, kw, cos, sin, positions, eps, interleaved);
-  return {y[0], y[1]};
+  Tensor yq, yk;
+  {
+    Below below;
+    std::tie(yq, yk) = qk_norm_rotary(q, k, qw, kw, cos, sin, positions, eps, interleaved);
+  }
+  if (node) {
+    torch::autograd::set_history(yq, node);
+    torch::autograd::set_history(yk, node);
+  }
+  return {yq, yk};
 }
 std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_backward(const Tensor& dyq, const Tensor& dyk, const Tensor& q, const Tensor& k,
                                                                    const OptTensor& qw, const OptTensor& kw, const Tensor& cos,
@@ -411,7 +444,7 @@ Tensor score_layout(const Tensor& t) {
 }
 Tensor in_layout_of(const Tensor& t, const Tensor& like) {
   if (t.strides() == like.strides() && sixteen(t)) return t;
-  return at::empty_strided(like.sizes(), like.strides(), like.options()).copy_(t);
+  return fresh_strided(like).copy_(t);
 }
 
 B200BiasSoftmax bias_params(const BiasArgs& a, const Tensor& scores, const Tensor& table) {
@@ -454,7 +487,7 @@ std::tuple<Tensor, Tensor> bias_fwd(const BiasArgs& a, Tensor& laid_out) {
   }
   OpScope scope("relative_bias_softmax", a.scores);
   Tensor s = laid_out = score_layout(a.scores), table = a.table.contiguous();
-  Tensor probs = at::empty_strided(s.sizes(), s.strides(), s.options()), stats = at::empty(ss, s.options().dtype(at::kFloat));
+  Tensor probs = fresh_strided(s), stats = fresh(ss, at::kFloat, s);
   B200BiasSoftmax p = bias_params(a, s, table);
   p.out = probs.data_ptr();
   p.stats = stats.data_ptr<float>();
@@ -486,13 +519,13 @@ std::tuple<Tensor, Tensor> bias_bwd(const BiasArgs& a, const Tensor& grad, const
   }
   OpScope scope(op, a.scores);
   Tensor s = score_layout(a.scores), g = in_layout_of(grad, s), table = a.table.contiguous();
-  Tensor ds = at::empty_strided(s.sizes(), s.strides(), s.options()), dt;
+  Tensor ds = fresh_strided(s), dt;
   B200BiasSoftmax p = bias_params(a, s, table);
   p.grad = g.data_ptr();
   p.out = ds.data_ptr();
   p.stats = stats.data_ptr<float>();
   if (need_table) {
-    dt = at::empty_like(table);
+    dt = fresh(table.sizes(), table);
     p.dtable = dt.data_ptr();
   }
   Workspace ws((size_t)b200_bias_softmax_workspace(&p), scope);
@@ -500,34 +533,27 @@ std::tuple<Tensor, Tensor> bias_bwd(const BiasArgs& a, const Tensor& grad, const
   return {ds, dt};
 }
 
-struct BiasFn : public torch::autograd::Function<BiasFn> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& scores, const Tensor& table, const OptTensor& mask, double scale,
-                               bool bidirectional, int64_t max_distance, int64_t query_offset) {
-    at::AutoDispatchBelowADInplaceOrView guard;
-    Tensor laid_out;
-    auto [probs, stats] = bias_fwd({scores, table, mask, scale, bidirectional, max_distance, query_offset}, laid_out);
-    ctx->save_for_backward({laid_out, table, given(mask) ? *mask : Tensor(), stats});
-    ctx->mark_non_differentiable({stats});
-    ctx->saved_data["scale"] = scale;
-    ctx->saved_data["bidirectional"] = bidirectional;
-    ctx->saved_data["max_distance"] = max_distance;
-    ctx->saved_data["query_offset"] = query_offset;
-    ctx->saved_data["need_table"] = table.requires_grad();
-    return {probs, stats};
+struct BiasNode : public torch::autograd::Node {
+  SavedVariable scores, table, mask, stats;
+  double scale = 1;
+  bool bidirectional = true;
+  int64_t max_distance = 0, query_offset = 0;
+  std::string name() const override { return "RelativeBiasSoftmaxBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* s : {&scores, &table, &mask, &stats}) s->reset_data();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const variable_list s = ctx->get_saved_variables();
-    variable_list out(7);
+  variable_list apply(variable_list&& g) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(2);
     if (!g[0].defined()) return out;
+    const Tensor s = scores.unpack(), t = table.unpack(), m = mask.unpack(), st = stats.unpack();
     {
-      at::AutoDispatchBelowADInplaceOrView guard;
-      at::NoGradGuard no_grad;
-      auto& d = ctx->saved_data;
-      auto [ds, dt] = bias_bwd({s[0], s[1], saved_optional(s[2]), d["scale"].toDouble(), d["bidirectional"].toBool(),
-                                d["max_distance"].toInt(), d["query_offset"].toInt()}, g[0], s[3], d["need_table"].toBool());
-      out[0] = ds; out[1] = dt;
+      Below below;
+      std::tie(out[0], out[1]) =
+          bias_bwd({s, t, saved_optional(m), scale, bidirectional, max_distance, query_offset}, g[0], st, task_should_compute_output(1));
     }
-    return once_differentiable("relative_bias_softmax", out);
+    return once_differentiable("relative_bias_softmax", std::move(out));
   }
 };
 
@@ -538,12 +564,19 @@ std::tuple<Tensor, Tensor> relative_bias_softmax(const Tensor& scores, const Ten
 }
 std::tuple<Tensor, Tensor> relative_bias_softmax_autograd(const Tensor& scores, const Tensor& table, const OptTensor& mask, double scale,
                                                           bool bidirectional, int64_t max_distance, int64_t query_offset) {
-  if (!wants_grad({&scores, &table})) {
-    at::AutoDispatchBelowADInplaceOrView guard;
-    return relative_bias_softmax(scores, table, mask, scale, bidirectional, max_distance, query_offset);
+  Tensor probs, stats, laid_out;
+  {
+    Below below;
+    std::tie(probs, stats) = bias_fwd({scores, table, mask, scale, bidirectional, max_distance, query_offset}, laid_out);
   }
-  const variable_list y = BiasFn::apply(scores, table, mask, scale, bidirectional, max_distance, query_offset);
-  return {y[0], y[1]};
+  if (wants_grad({&scores, &table})) {
+    auto node = make_node<BiasNode>();
+    node->set_next_edges(torch::autograd::collect_next_edges(scores, table));
+    node->scores = save(laid_out); node->table = save(table); node->mask = save(or_none(mask)); node->stats = save(stats);
+    node->scale = scale; node->bidirectional = bidirectional; node->max_distance = max_distance; node->query_offset = query_offset;
+    torch::autograd::set_history(probs, node);
+  }
+  return {probs, stats};
 }
 std::tuple<Tensor, Tensor> relative_bias_softmax_backward(const Tensor& grad, const Tensor& scores, const Tensor& stats, const Tensor& table,
                                                           const OptTensor& mask, double scale, bool bidirectional, int64_t max_distance,
@@ -617,8 +650,8 @@ Tensor row_layout(const Tensor& t) {
 Tensor empty_in_phase(const Tensor& t, int64_t ld) {
   const int64_t phase = (int64_t)(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) / (int64_t)t.element_size();
   const int64_t rows = t.size(0), need = rows > 0 ? (rows - 1) * ld + t.size(1) : 0;
-  if (phase == 0 && ld == t.size(1)) return at::empty(t.sizes(), t.options());
-  return at::empty({need + phase}, t.options()).as_strided(t.sizes(), {ld, 1}, phase);
+  if (phase == 0 && ld == t.size(1)) return fresh(t.sizes(), t);
+  return fresh({need + phase}, t).as_strided(t.sizes(), {ld, 1}, phase);
 }
 
 B200Distill distill_params(const DistillArgs& a, const Tensor& z, const Tensor& teacher, const Tensor& index) {
@@ -656,8 +689,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> distill_fwd(const DistillArgs& a, boo
   }
   OpScope scope("top_logits_distillation", a.logits);
   Tensor z = row_layout(a.logits), teacher = a.teacher.contiguous(), index = a.index.contiguous();
-  Tensor rows = at::empty({N}, fopt), stats = at::empty({N, 2}, fopt), count = at::empty({2}, fopt);  // (count, scratch)
-  Tensor loss = each ? rows : at::empty({}, fopt), grad;
+  Tensor rows = fresh({N}, at::kFloat, z), stats = fresh({N, 2}, at::kFloat, z), count = fresh({2}, at::kFloat, z);  // (count, scratch)
+  Tensor loss = each ? rows : fresh({}, at::kFloat, z), grad;
   B200Distill p = distill_params(a, z, teacher, index);
   p.row_loss = rows.data_ptr<float>();
   p.stats = stats.data_ptr<float>();
@@ -704,35 +737,27 @@ Tensor distill_bwd(const DistillArgs& a, const Tensor& grad, const Tensor& stats
   return out;
 }
 
-struct DistillFn : public torch::autograd::Function<DistillFn> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature,
-                               int64_t reduction) {
-    at::AutoDispatchBelowADInplaceOrView guard;
-    auto [loss, stats, count, ready] = distill_fwd({logits, teacher, index, temperature, reduction}, true);
-    ctx->save_for_backward({logits, teacher, index, stats, count});
-    ctx->saved_data["temperature"] = temperature;
-    ctx->saved_data["reduction"] = reduction;
-    if (ready.defined()) ctx->saved_data["ready"] = ready;
-    return {loss};
+struct DistillNode : public torch::autograd::Node {
+  SavedVariable logits, teacher, index, stats, count;
+  Tensor ready;  // the gradient for a factor of 1, handed out once: a second pass over a retained graph writes one of its own
+  double temperature = 1;
+  int64_t reduction = 0;
+  std::string name() const override { return "TopLogitsDistillationBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* s : {&logits, &teacher, &index, &stats, &count}) s->reset_data();
+    ready = Tensor();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const variable_list s = ctx->get_saved_variables();
-    variable_list out(5);
+  variable_list apply(variable_list&& g) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(1);
     if (!g[0].defined()) return out;
+    const Tensor z = logits.unpack(), t = teacher.unpack(), i = index.unpack(), st = stats.unpack(), n = count.unpack();
     {
-      at::AutoDispatchBelowADInplaceOrView guard;
-      at::NoGradGuard no_grad;
-      // handed out once: a second pass over a retained graph writes a gradient of its own
-      Tensor ready;
-      auto it = ctx->saved_data.find("ready");
-      if (it != ctx->saved_data.end()) {
-        ready = it->second.toTensor();
-        ctx->saved_data.erase("ready");
-      }
-      out[0] = distill_bwd({s[0], s[1], s[2], ctx->saved_data["temperature"].toDouble(), ctx->saved_data["reduction"].toInt()}, g[0], s[3],
-                           s[4], ready);
+      Below below;
+      out[0] = distill_bwd({z, t, i, temperature, reduction}, g[0], st, n, std::exchange(ready, Tensor()));
     }
-    return once_differentiable("top_logits_distillation", out);
+    return once_differentiable("top_logits_distillation", std::move(out));
   }
 };
 
@@ -741,11 +766,22 @@ Tensor top_logits_distillation(const Tensor& logits, const Tensor& teacher, cons
 }
 Tensor top_logits_distillation_autograd(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature,
                                         int64_t reduction) {
-  if (!wants_grad({&logits})) {
-    at::AutoDispatchBelowADInplaceOrView guard;
-    return top_logits_distillation(logits, teacher, index, temperature, reduction);
+  const bool grad = wants_grad({&logits});
+  Tensor loss, stats, count, ready;
+  {
+    Below below;
+    std::tie(loss, stats, count, ready) = distill_fwd({logits, teacher, index, temperature, reduction}, grad);
   }
-  return DistillFn::apply(logits, teacher, index, temperature, reduction)[0];
+  if (grad) {
+    auto node = make_node<DistillNode>();
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    node->logits = save(logits); node->teacher = save(teacher); node->index = save(index); node->stats = save(stats); node->count = save(count);
+    node->ready = ready;
+    node->temperature = temperature;
+    node->reduction = reduction;
+    torch::autograd::set_history(loss, node);
+  }
+  return loss;
 }
 
 }  // namespace

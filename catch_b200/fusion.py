@@ -411,7 +411,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     ``[positions, rotated / 2]`` rotate the first ``rotated`` dimensions in pairs ``(i, i + rotated / 2)``, or ``(2i, 2i + 1)`` with
     ``interleaved``; the other dimensions are normalised only.  ``positions`` (int64 / int32, ``[batch, length]`` or ``[length]``)
     chooses the rows of the tables, by default ``0 .. length - 1``; a token whose position lies outside them (a padding token
-    marked with -1) gives zeros and gets zero gradients.  The results are contiguous and have the inputs' dtype; sums are taken in
+    marked with -1) gives zeros and gets zero gradients; in synchronous mode a position behind the tables raises.  The results are contiguous and have the inputs' dtype; sums are taken in
     fp32.  Differentiable in ``q``, ``k`` and the weights."""
     return torch.ops.catch_b200.qk_norm_rotary.default(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 

@@ -5,7 +5,10 @@ The reference lists BERT among the networks it trains
 (docs/user_guide/source/pytorch_8_training/Pytorch_training.rst:10-18) with plain
 matmul / bmm / softmax eager ops; this definition uses exactly those ops (embedding,
 LayerNorm, linear, bmm, softmax, GELU, dropout), all of which have kernels in this
-backend.
+backend.  ``BertConfig.position_embedding_type`` chooses how tokens learn of their places:
+``"absolute"`` (embeddings, the default), ``"relative_bias"`` (a learned bias of the scores by
+relative position, one table for each layer) or ``"rotary"`` (queries and keys are normalised
+and rotated by position).
 """
 from __future__ import annotations
 
@@ -29,13 +32,19 @@ class BertConfig:
     attention_probs_dropout_prob: float = 0.1
     layer_norm_eps: float = 1e-12
     num_labels: int = 2
+    position_embedding_type: str = "absolute"   # or "relative_bias", "rotary"
+    relative_attention_num_buckets: int = 32
+    relative_attention_max_distance: int = 128
+    rotary_base: float = 10000.0
 
 
 class BertEmbeddings(nn.Module):
     def __init__(self, c: BertConfig):
         super().__init__()
         self.word_embeddings = nn.Embedding(c.vocab_size, c.hidden_size)
-        self.position_embeddings = nn.Embedding(c.max_position_embeddings, c.hidden_size)
+        self.absolute = c.position_embedding_type == "absolute"
+        if self.absolute:
+            self.position_embeddings = nn.Embedding(c.max_position_embeddings, c.hidden_size)
         self.token_type_embeddings = nn.Embedding(c.type_vocab_size, c.hidden_size)
         self.LayerNorm = nn.LayerNorm(c.hidden_size, eps=c.layer_norm_eps)
         self.dropout = nn.Dropout(c.hidden_dropout_prob)
@@ -45,8 +54,11 @@ class BertEmbeddings(nn.Module):
         L = input_ids.shape[1]
         if token_type_ids is None:
             token_type_ids = torch.zeros_like(input_ids)
-        x = (self.word_embeddings(input_ids) + self.position_embeddings(self.position_ids[:, :L]) +
-             self.token_type_embeddings(token_type_ids))
+        if self.absolute:
+            x = (self.word_embeddings(input_ids) + self.position_embeddings(self.position_ids[:, :L]) +
+                 self.token_type_embeddings(token_type_ids))
+        else:
+            x = self.word_embeddings(input_ids) + self.token_type_embeddings(token_type_ids)
         return self.dropout(self.LayerNorm(x))
 
 
@@ -58,19 +70,53 @@ class BertSelfAttention(nn.Module):
         self.key = nn.Linear(c.hidden_size, c.hidden_size)
         self.value = nn.Linear(c.hidden_size, c.hidden_size)
         self.dropout = nn.Dropout(c.attention_probs_dropout_prob)
+        self.position = c.position_embedding_type
+        if self.position == "relative_bias":
+            self.max_distance = c.relative_attention_max_distance
+            self.relative_bias = nn.Parameter(torch.zeros(c.relative_attention_num_buckets, self.h))
+        elif self.position == "rotary":
+            self.query_norm = nn.Parameter(torch.ones(self.d))
+            self.key_norm = nn.Parameter(torch.ones(self.d))
+            angle = torch.arange(c.max_position_embeddings, dtype=torch.float64)[:, None] * (
+                c.rotary_base ** (-torch.arange(0, self.d, 2, dtype=torch.float64) / self.d))
+            self.register_buffer("rotary_cos", angle.cos().float(), persistent=False)
+            self.register_buffer("rotary_sin", angle.sin().float(), persistent=False)
+        elif self.position != "absolute":
+            raise ValueError(f"position_embedding_type must be 'absolute', 'relative_bias' or 'rotary', got {self.position!r}")
+
+    def _project(self, x):
+        """Queries, keys and values as [B, L, h, d], the first two rotated by position where the model does that."""
+        B, L, _ = x.shape
+        q, k, v = (p(x).view(B, L, self.h, self.d) for p in (self.query, self.key, self.value))
+        if self.position == "rotary":
+            from catch_b200.fusion import qk_norm_rotary
+
+            q, k = qk_norm_rotary(q, k, self.query_norm, self.key_norm, self.rotary_cos, self.rotary_sin)
+        return q, k, v
+
+    def _biased_probs(self, scores, mask):
+        """Softmax of unscaled [B, h, L, L] scores with the relative position bias."""
+        from catch_b200.fusion import relative_bias_softmax
+
+        return relative_bias_softmax(scores, self.relative_bias, mask, scale=1.0 / math.sqrt(self.d), max_distance=self.max_distance)
 
     def forward(self, x, mask=None):
         B, L, H = x.shape
 
-        def split(t):  # [B, L, H] -> [B*h, L, d]
-            return t.view(B, L, self.h, self.d).permute(0, 2, 1, 3).reshape(B * self.h, L, self.d)
+        def split(t):  # [B, L, h, d] -> [B*h, L, d]
+            return t.permute(0, 2, 1, 3).reshape(B * self.h, L, self.d)
 
-        q, k, v = split(self.query(x)), split(self.key(x)), split(self.value(x))
-        scores = torch.bmm(q, k.transpose(1, 2)) * (1.0 / math.sqrt(self.d))
-        if mask is not None:
-            scores = scores.view(B, self.h, L, L) + mask
-            scores = scores.view(B * self.h, L, L)
-        probs = self.dropout(torch.softmax(scores, dim=-1))
+        q, k, v = (split(t) for t in self._project(x))
+        scores = torch.bmm(q, k.transpose(1, 2))
+        if self.position == "relative_bias":
+            probs = self._biased_probs(scores.view(B, self.h, L, L), mask).view(B * self.h, L, L)
+        else:
+            scores = scores * (1.0 / math.sqrt(self.d))
+            if mask is not None:
+                scores = scores.view(B, self.h, L, L) + mask
+                scores = scores.view(B * self.h, L, L)
+            probs = torch.softmax(scores, dim=-1)
+        probs = self.dropout(probs)
         ctx = torch.bmm(probs, v).view(B, self.h, L, self.d).permute(0, 2, 1, 3).reshape(B, L, H)
         return ctx
 
@@ -104,15 +150,18 @@ class FusedBertSelfAttention(BertSelfAttention):
         B, L, H = x.shape
         cd = torch.get_autocast_dtype("blackwell")
 
-        def heads(t):  # [B, L, H] -> [B, h, L, d] view
-            return t.to(cd).view(B, L, self.h, self.d).permute(0, 2, 1, 3)
+        def heads(t):  # [B, L, h, d] -> [B, h, L, d] view
+            return t.to(cd).permute(0, 2, 1, 3)
 
-        q, k, v = heads(self.query(x)), heads(self.key(x)), heads(self.value(x))
-        scores = matmul_nd(q, k.transpose(-1, -2), 1.0 / math.sqrt(self.d))
-        if mask is not None:
-            scores = scores + mask.to(scores.dtype)
-        with torch.autocast("blackwell", enabled=False):  # the softmax kernel computes in fp32 whatever the storage type
-            probs = torch.softmax(scores, dim=-1)
+        q, k, v = (heads(t) for t in self._project(x))
+        if self.position == "relative_bias":
+            probs = self._biased_probs(matmul_nd(q, k.transpose(-1, -2)), mask)  # scale, bias, mask and softmax in one kernel
+        else:
+            scores = matmul_nd(q, k.transpose(-1, -2), 1.0 / math.sqrt(self.d))
+            if mask is not None:
+                scores = scores + mask.to(scores.dtype)
+            with torch.autocast("blackwell", enabled=False):  # the softmax kernel computes in fp32 whatever the storage type
+                probs = torch.softmax(scores, dim=-1)
         probs = self.dropout(probs)
         # the context is produced straight in [B, L, h, d] memory, seen as [B, h, L, d] by the product
         ctx = matmul_nd(probs, v, 1.0, (L * H, self.d, H, 1))

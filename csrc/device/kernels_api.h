@@ -545,7 +545,7 @@ typedef struct B200QkNormRotary {
   const float* sin;
   int64_t table_rows;
   const void* positions;     // [B, L] of int64 / int32 with pos_stride, or null: 0 .. L-1.  Outside the tables: zeros are
-  int positions_dtype;       // written for the token and *bad_flag is set
+  int positions_dtype;       // written for the token, and behind them *bad_flag is set
   int64_t pos_stride[2];
   int* bad_flag;             // may be null
   float eps;

@@ -43,7 +43,7 @@ struct Args {
   long long pos_b, pos_l;
   int pos_is_64;
   long long table_rows;
-  int* bad_flag;        // set when a position lies outside the tables; may be null
+  int* bad_flag;        // set when a position lies behind the tables; may be null
   unsigned L;
   int D, R, group;      // lanes per head
   float eps;
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(CH, BWD)) qk_norm_ro
       pos = p.pos_is_64 ? static_cast<const long long*>(p.positions)[at] : (long long)static_cast<const int*>(p.positions)[at];
     }
     const bool inside = now.hn > 0 && pos >= 0 && pos < p.table_rows;
-    if (now.hn > 0 && !inside && p.bad_flag && gl == 0) *p.bad_flag = 1;
+    if (now.hn > 0 && pos >= p.table_rows && p.bad_flag && gl == 0) *p.bad_flag = 1;
     float cs[CH][VEC], sn[CH][VEC];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {

@@ -19,6 +19,7 @@
 #include <map>
 #include <mutex>
 
+#include "../runtime/graph.h"
 #include "common.h"
 #include "kernels.h"
 
@@ -111,7 +112,7 @@ std::tuple<Tensor, Tensor, Tensor> host_angles(const RotaryArgs& a) {
   Tensor pos = positions_of(a).to(at::kLong);
   Tensor inside = pos.ge(0).logical_and(pos.lt(a.cos.size(0)));
   if (flags().async_disable && pos.numel() > 0)
-    TORCH_CHECK_INDEX(inside.all().item<bool>(), "qk_norm_rotary: index out of range");
+    TORCH_CHECK_INDEX(pos.lt(a.cos.size(0)).all().item<bool>(), "qk_norm_rotary: index out of range");
   std::vector<int64_t> shape{pos.size(0), pos.size(1), 1, a.cos.size(1)};
   Tensor cos = at::zeros(shape, a.q.options().dtype(at::kFloat)), sin = at::zeros(shape, a.q.options().dtype(at::kFloat));
   if (a.cos.size(0) > 0) {
@@ -260,6 +261,17 @@ struct Below {
   at::NoGradGuard no_grad;
 };
 
+// Autograd runs a backward on a thread of its own, whose memory does not come from the pool of a graph that the caller is capturing:
+// a replay would write to memory that belongs to others by then.  The operators' _backward forms, called by the capturing thread, are fine.
+void refuse_captured_backward(const char* op, const Tensor& t) {
+  if (!on_device(t) || graphCaptureActive()) return;
+  void* queue = getCurrentQueue(t.device().index()).handle();
+  int capturing = 0;
+  if (queue) TORCH_CHECK(b200_stream_is_capturing(queue, &capturing) == 0, op, ": the queue cannot be asked whether it is captured");
+  TORCH_CHECK(!capturing, op, ": a backward pass through autograd cannot be captured into a device graph; capture torch.ops.catch_b200.", op,
+              "_backward instead");
+}
+
 struct RotaryNode : public torch::autograd::Node {
   SavedVariable q, k, qw, kw, cos, sin, positions;
   double eps = 0;
@@ -274,6 +286,7 @@ struct RotaryNode : public torch::autograd::Node {
     variable_list out(4);
     if (!g[0].defined() && !g[1].defined()) return out;
     const Tensor uq = q.unpack(), uk = k.unpack();
+    refuse_captured_backward("qk_norm_rotary", uq);
     {
       Below below;
       Tensor gq = g[0].defined() ? g[0] : at::zeros_like(uq, at::MemoryFormat::Contiguous);
@@ -548,6 +561,7 @@ struct BiasNode : public torch::autograd::Node {
     variable_list out(2);
     if (!g[0].defined()) return out;
     const Tensor s = scores.unpack(), t = table.unpack(), m = mask.unpack(), st = stats.unpack();
+    refuse_captured_backward("relative_bias_softmax", s);
     {
       Below below;
       std::tie(out[0], out[1]) =
@@ -753,6 +767,7 @@ struct DistillNode : public torch::autograd::Node {
     variable_list out(1);
     if (!g[0].defined()) return out;
     const Tensor z = logits.unpack(), t = teacher.unpack(), i = index.unpack(), st = stats.unpack(), n = count.unpack();
+    refuse_captured_backward("top_logits_distillation", z);
     {
       Below below;
       out[0] = distill_bwd({z, t, i, temperature, reduction}, g[0], st, n, std::exchange(ready, Tensor()));
@@ -763,6 +778,15 @@ struct DistillNode : public torch::autograd::Node {
 
 Tensor top_logits_distillation(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction) {
   return std::get<0>(distill_fwd({logits, teacher, index, temperature, reduction}, false));
+}
+std::tuple<Tensor, Tensor, Tensor> top_logits_distillation_stats(const Tensor& logits, const Tensor& teacher, const Tensor& index,
+                                                                 double temperature, int64_t reduction) {
+  auto [loss, stats, count, ready] = distill_fwd({logits, teacher, index, temperature, reduction}, false);
+  return {loss, stats, count};
+}
+Tensor top_logits_distillation_backward(const Tensor& grad, const Tensor& logits, const Tensor& stats, const Tensor& count, const Tensor& teacher,
+                                        const Tensor& index, double temperature, int64_t reduction) {
+  return distill_bwd({logits, teacher, index, temperature, reduction}, grad, stats, count, Tensor());
 }
 Tensor top_logits_distillation_autograd(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature,
                                         int64_t reduction) {
@@ -799,9 +823,16 @@ TORCH_LIBRARY_FRAGMENT(catch_b200, m) {
   // reduction: 0 a loss for each row, 1 their mean over the rows with entries, 2 their sum
   m.def("top_logits_distillation(Tensor logits, Tensor teacher_logits, Tensor teacher_index, float temperature=1.0, int reduction=1) "
         "-> Tensor");
+  // the loss with what its backward needs (statistics of the rows, number of rows that count), and that backward
+  m.def("top_logits_distillation_stats(Tensor logits, Tensor teacher_logits, Tensor teacher_index, float temperature, int reduction) "
+        "-> (Tensor, Tensor, Tensor)");
+  m.def("top_logits_distillation_backward(Tensor grad, Tensor logits, Tensor stats, Tensor count, Tensor teacher_logits, "
+        "Tensor teacher_index, float temperature, int reduction) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(catch_b200, CompositeExplicitAutograd, m) {
+  m.impl("top_logits_distillation_stats", TORCH_FN(top_logits_distillation_stats));
+  m.impl("top_logits_distillation_backward", TORCH_FN(top_logits_distillation_backward));
   m.impl("qk_norm_rotary", TORCH_FN(qk_norm_rotary));
   m.impl("qk_norm_rotary_backward", TORCH_FN(qk_norm_rotary_backward));
   m.impl("relative_bias_softmax", TORCH_FN(relative_bias_softmax));

@@ -134,3 +134,52 @@ def test_bucket_borders_are_exact(buckets, bidirectional, max_distance):
     p = p.flatten().double().log()
     got = ((p - p[far]) * buckets).round().long() + want[far]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dev", ["cpu", "blackwell"])
+def test_gradients_against_differences(dev):
+    from transformer_op_checks import differences
+
+    differences(dev)
+
+
+@pytest.mark.parametrize("position", ["absolute", "relative_bias", "rotary"])
+@pytest.mark.parametrize("fused", [False, True])
+def test_a_student_learns_from_a_teacher(position, fused):
+    from transformer_op_checks import student_step
+
+    student_step("blackwell", position, fused)
+
+
+def test_position_types_of_the_encoder():
+    from catch_b200.models.bert import BertConfig, BertForSequenceClassification
+
+    small = dict(vocab_size=50, hidden_size=16, num_hidden_layers=1, num_attention_heads=2, intermediate_size=32, max_position_embeddings=10)
+    names = {t: set(BertForSequenceClassification(BertConfig(position_embedding_type=t, **small)).state_dict()) for t in
+             ("absolute", "relative_bias", "rotary")}
+    assert names["absolute"] == set(BertForSequenceClassification(BertConfig(**small)).state_dict())
+    base = names["absolute"] - {"embeddings.position_embeddings.weight"}
+    assert names["relative_bias"] == base | {"layers.0.attention.relative_bias"}
+    assert names["rotary"] == base | {"layers.0.attention.query_norm", "layers.0.attention.key_norm"}
+    with pytest.raises(ValueError, match="position_embedding_type"):
+        BertForSequenceClassification(BertConfig(position_embedding_type="learned", **small))
+    with pytest.raises(RuntimeError, match="12 tokens, but cos and sin have 10 positions"):
+        BertForSequenceClassification(BertConfig(position_embedding_type="rotary", **small))(torch.zeros(1, 12, dtype=torch.long))
+
+
+def test_an_index_out_of_range_raises_in_synchronous_mode():
+    from catch_b200.fusion import qk_norm_rotary, top_logits_distillation
+
+    cos, sin = cases.tables(4, 4)
+    q = torch.randn(1, 3, 2, 8)
+    torch.b200.set_flag("async_disable", True)
+    try:
+        with pytest.raises(IndexError, match="qk_norm_rotary"):
+            qk_norm_rotary(q, q, None, None, cos, sin, torch.tensor([[0, 1, 4]]))
+        with pytest.raises(IndexError, match="top_logits_distillation"):
+            top_logits_distillation(torch.randn(2, 5), torch.randn(2, 2), torch.tensor([[0, 1], [2, 5]]))
+        y, _ = qk_norm_rotary(q, q, None, None, cos, sin, torch.tensor([[-1, 0, 3]]))  # padding
+        assert y[0, 0].abs().max() == 0 and y[0, 1].abs().max() > 0
+        top_logits_distillation(torch.randn(2, 5), torch.randn(2, 2), torch.tensor([[0, -1], [-100, 4]]))
+    finally:
+        torch.b200.set_flag("async_disable", False)

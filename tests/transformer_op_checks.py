@@ -269,3 +269,98 @@ OPS_CHECKS = _entries()
 def run_check(name, dev):
     fn, kw, _ = OPS_CHECKS[name]
     fn(dev, **kw)
+
+
+# ------------------------------------------------------------------------------------------ gradients against differences
+def against_differences(f, x, grad, step, what):
+    """``f`` (a number from fp32 tensors, summed in 64 bits) along three directions: the central difference is off by step^2 / 6 times
+    the third derivative and by the rounding of f's fp32 results over the step; the functions here are sums of some hundred terms of
+    size one with derivatives of size one, so 2^-8 relative to the gradient's length covers both at a step of 2^-7."""
+    g = torch.Generator().manual_seed(5)
+    for _ in range(3):
+        v = torch.randn(x.shape, generator=g)
+        v = v / v.norm()
+        dev = v.to(x.device)
+        slope = (f(x + step * dev) - f(x - step * dev)) / (2 * step)
+        want = float((grad.detach().cpu().double() * v.double()).sum())
+        assert abs(slope - want) <= 2.0 ** -8 * max(1.0, float(grad.detach().cpu().double().norm())), (what, slope, want)
+
+
+def differences(dev):
+    from catch_b200.fusion import qk_norm_rotary, relative_bias_softmax, top_logits_distillation
+
+    torch.manual_seed(8)
+    h = 2.0 ** -7
+    total = lambda t, g: float((t.detach().cpu().double() * g.double()).sum())  # noqa: E731
+    q, k, w = torch.randn(1, 3, 2, 8).to(dev), torch.randn(1, 3, 1, 8).to(dev), (1 + 0.2 * torch.randn(8)).to(dev)
+    cos, sin = (t.to(dev) for t in cases.tables(3, 6))
+    gq, gk = torch.randn(1, 3, 2, 8), torch.randn(1, 3, 1, 8)
+    rot = lambda q, k, w: (lambda y: total(y[0], gq) + total(y[1], gk))(qk_norm_rotary(q, k, w, w, cos, sin))  # noqa: E731
+    leaves = [t.clone().requires_grad_() for t in (q, k, w)]
+    y = qk_norm_rotary(leaves[0], leaves[1], leaves[2], leaves[2], cos, sin)
+    grads = torch.autograd.grad(y, leaves, (gq.to(dev), gk.to(dev)))
+    for i, (t, g) in enumerate(zip((q, k, w), grads)):
+        against_differences(lambda x: rot(*[x if j == i else o for j, o in enumerate((q, k, w))]), t, g, h, f"rotary {i}")
+    s, t = torch.randn(2, 2, 5, 6).to(dev), torch.randn(4, 2).to(dev)
+    m = torch.ones(2, 1, 5, 6, dtype=torch.bool)
+    m[:, :, :, 4:] = False
+    m[0, 0, 1] = False
+    gp = torch.randn(2, 2, 5, 6)
+    soft = lambda s, t: relative_bias_softmax(s, t, m.to(dev), scale=0.7, max_distance=6)  # noqa: E731
+    sl, tl = s.clone().requires_grad_(), t.clone().requires_grad_()
+    ds, dt = torch.autograd.grad(soft(sl, tl), (sl, tl), gp.to(dev))
+    against_differences(lambda x: total(soft(x, t), gp), s, ds, h, "scores")
+    against_differences(lambda x: total(soft(s, x), gp), t, dt, h, "table")
+    z = torch.randn(4, 11).to(dev)
+    te, idx = cases.teacher_of(4, 11, 3, 2)
+    idx[0, 1] = -1
+    loss = lambda z: top_logits_distillation(z, te.to(dev), idx.to(dev), temperature=1.5, reduction="sum")  # noqa: E731
+    zl = z.clone().requires_grad_()
+    (dz,) = torch.autograd.grad(loss(zl), zl)
+    against_differences(lambda x: float(loss(x)), z, dz, h, "logits")
+
+
+# -------------------------------------------------------------------------------------------------------- together
+def _student(position, layers=2):
+    from catch_b200.models.bert import BertConfig, BertForSequenceClassification
+
+    torch.manual_seed(3)
+    c = BertConfig(vocab_size=97, hidden_size=32, num_hidden_layers=layers, num_attention_heads=4, intermediate_size=64,
+                   max_position_embeddings=40, num_labels=24, hidden_dropout_prob=0.0, attention_probs_dropout_prob=0.0,
+                   position_embedding_type=position)
+    m = BertForSequenceClassification(c)
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            if "relative_bias" in n or n.endswith("_norm"):  # (not the places where their gradients would say nothing)
+                p.add_(0.3 * torch.randn_like(p))
+    return m
+
+
+def student_step(dev, position, fused=False, dtype=None):
+    """An encoder with the model's own switch for positions learns from a teacher's top logits: loss and gradients of one step, on
+    ``dev`` and with plain modules on the host."""
+    from catch_b200.fusion import top_logits_distillation
+    from catch_b200.models.bert import fuse_bert
+
+    torch.manual_seed(4)
+    ids = torch.randint(0, 97, (3, 17))
+    keep = torch.ones(3, 17)
+    keep[1, 9:] = 0
+    te, idx = cases.teacher_of(3, 24, 5, 1)
+
+    def step(model, d, autocast):
+        with torch.autocast(d.split(":")[0], dtype=dtype or torch.bfloat16, enabled=autocast):
+            logits = model(ids.to(d), attention_mask=keep.to(d))
+        loss = top_logits_distillation(logits, te.to(d), idx.to(d), temperature=2.0)
+        loss.backward()
+        return float(loss.detach()), {n: p.grad.detach().cpu().double() for n, p in model.named_parameters() if p.grad is not None}
+
+    ref_loss, ref = step(_student(position), "cpu", False)
+    model = _student(position).to(dev)
+    got_loss, got = step(fuse_bert(model) if fused else model, dev, dtype is not None)
+    assert set(got) == set(ref) and any("relative_bias" in n or n.endswith("_norm") for n in got) == (position != "absolute")
+    # products of the device: TF32 (2^-11 a factor) or 16 bits (2^-8), through some twenty products in a row either way
+    tol = 20 * 2 * (2.0 ** -11 if dtype is None else 2.0 ** -8)
+    assert abs(got_loss - ref_loss) <= tol * abs(ref_loss)
+    for n in ref:
+        assert (got[n] - ref[n]).norm() <= tol * ref[n].norm() + 1e-6, (n, float((got[n] - ref[n]).norm() / ref[n].norm()))

@@ -39,6 +39,8 @@ class BertConfig:
 
 
 class BertEmbeddings(nn.Module):
+    absolute = True  # (also for modules that were pickled before there was a choice)
+
     def __init__(self, c: BertConfig):
         super().__init__()
         self.word_embeddings = nn.Embedding(c.vocab_size, c.hidden_size)
@@ -63,6 +65,8 @@ class BertEmbeddings(nn.Module):
 
 
 class BertSelfAttention(nn.Module):
+    position = "absolute"
+
     def __init__(self, c: BertConfig):
         super().__init__()
         self.h, self.d = c.num_attention_heads, c.hidden_size // c.num_attention_heads

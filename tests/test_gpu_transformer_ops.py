@@ -228,3 +228,9 @@ def test_logits_and_heads_beyond_two_to_the_31():
     dq = ops.qk_norm_rotary_backward(y, k, q, k, None, None, cos, sin, None, 1e-6, False)[0]
     part_dq = ops.qk_norm_rotary_backward(part, kf, few, kf, None, None, cos[-4:], sin[-4:], None, 1e-6, False)[0]
     assert torch.equal(dq[-1, -4:].cpu(), part_dq[0].cpu())
+
+
+def test_the_guide_executes():
+    from transformer_op_checks import guide
+
+    guide()

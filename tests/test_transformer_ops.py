@@ -183,3 +183,9 @@ def test_an_index_out_of_range_raises_in_synchronous_mode():
         top_logits_distillation(torch.randn(2, 5), torch.randn(2, 2), torch.tensor([[0, -1], [-100, 4]]))
     finally:
         torch.b200.set_flag("async_disable", False)
+
+
+def test_the_guide_executes():
+    from transformer_op_checks import guide
+
+    guide()

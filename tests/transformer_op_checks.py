@@ -364,3 +364,15 @@ def student_step(dev, position, fused=False, dtype=None):
     assert abs(got_loss - ref_loss) <= tol * abs(ref_loss)
     for n in ref:
         assert (got[n] - ref[n]).norm() <= tol * ref[n].norm() + 1e-6, (n, float((got[n] - ref[n]).norm() / ref[n].norm()))
+
+
+def guide():
+    """The code of docs/training.md on positions and distillation, run as written."""
+    from pathlib import Path
+
+    text = (Path(__file__).resolve().parent.parent / "docs" / "training.md").read_text()
+    code = text.split("## Positions in attention, learning from a teacher")[1].split("```python")[1].split("```")[0]
+    names = {}
+    exec(compile(code, "docs/training.md", "exec"), names)
+    for leaf in ("qkv", "norm", "table"):
+        assert bool(torch.isfinite(names[leaf].grad.float().cpu()).all()) and float(names[leaf].grad.float().cpu().abs().sum()) > 0

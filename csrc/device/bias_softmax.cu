@@ -9,14 +9,16 @@
 // so a block, which works on one head, keeps the 2 reach + 1 values it can take in shared memory.  The backward recomputes p from s
 // and two numbers a row (maximum and 1 / sum, fp32): reading s costs what reading p would, and p is not rounded in between.
 //
-// Table gradient: d is summed over distances first.  Far distances go to two registers a thread; near ones to shared memory, in a copy
-// for every group of lanes that walks over rows of its own.  In one row no two elements have the same distance, so no atomics
-// are needed and the order of every sum is fixed: the same inputs give the same bits.
+// Table gradient: d is summed over distances first, far ones in two registers a thread, near ones in shared memory, in a copy for every
+// group of lanes that walks over rows of its own.  In one row no two elements have the same distance, so no atomics are needed and the order
+// of every sum is fixed: the same inputs give the same bits.  From one row to the next a lane's distances fall by one, so its sums
+// stay in registers and move up a place, and one of eight reaches shared memory (16 x 12 x 512 x 512 bf16: 91 us when all did, 72 so).
 //
-// Measured on a B200, 2 x 12 x 2048 x 2048 bf16: without a mask forward 80 us = 5.0 TB/s, 0.76 of the measured copy bandwidth, backward (scores
-// alone) 111 us = 5.4 TB/s, 0.83; with a causal mask of 16 bits 116 and 160 us.  128 x 12 x 128 x 128 bf16 with an fp32 padding mask: 36 and
-// 50 us (2.8 and 3.0 TB/s), where every distance is a near one.  Issue slots are what it runs out of (68 % and 63 % busy at 2048 keys; 18 and 23
-// instructions an element), and unaligned fp32 rows of 517 keys with a random bool mask run at 1.4 TB/s for the same reason.
+// Measured on a B200, 2 x 12 x 2048 x 2048 bf16: without a mask forward 81 us = 5.0 TB/s, 0.76 of the measured copy bandwidth, backward 113 us for
+// the scores alone and 118 us with the table = 5.1 TB/s, 0.78; with a causal mask of 16 bits 117 and 180 us.  128 x 12 x 128 x 128 bf16 with an
+// fp32 padding mask: 38 and 70 us (2.6 and 2.1 TB/s), where every distance is a near one.  Issue slots are what it runs out of (68 % and 63 %
+// busy at 2048 keys; 18 and 23 instructions an element), and unaligned fp32 rows of 517 keys with a random bool mask run at 1.2 to 1.5 TB/s
+// for the same reason.
 #include "kernels_api.h"
 #include "row_vec.cuh"
 
@@ -265,6 +267,13 @@ __device__ __forceinline__ void add_distances(float* acc, int last, int x0, cons
   }
 }
 
+// One sum of a distance to where it belongs.
+__device__ __forceinline__ void add_distance(float* acc, int last, int x, float v, float& below, float& above) {
+  if (x <= 0) below += v;
+  else if (x >= last) above += v;
+  else acc[padded(x)] += v;
+}
+
 // Walks over the rows (b, i) of a head.
 struct RowWalk {
   unsigned i;
@@ -341,14 +350,18 @@ struct RowVectors {
   }
 };
 
-// Registers: 64 a thread forward and 80 backward hold 16 elements of a lane and leave 1024 and 768 threads for an SM.  Left alone, the
-// compiler takes 120 for the loads of a mask whose keys are not side by side, which is the rare case.
-constexpr int row_threads(int warps) { return warps == 1 ? kMaxThreads : 32 * warps; }
-constexpr int row_blocks(int elements, int warps, int resident) { return elements <= 16 ? resident / row_threads(warps) : 1; }
+// Registers: 64 a thread forward hold 16 elements of a lane and leave 1024 threads for an SM, 80 backward 768; where a row belongs to a
+// part of a warp 96 and 640, in smaller blocks.  Left alone, the compiler takes 120 for the loads of a mask whose keys are not side by
+// side, which is the rare case.
+constexpr int row_threads(int warps, bool bwd) { return warps == 1 ? (bwd ? 128 : kMaxThreads) : 32 * warps; }
+constexpr int resident_threads(int warps, bool bwd) { return bwd ? (warps == 1 ? 640 : 768) : 1024; }
+constexpr int row_blocks(int elements, int warps, bool bwd) {
+  return elements <= 16 ? resident_threads(warps, bwd) / row_threads(warps, bwd) : 1;
+}
 
 // A row in registers: NV vectors of VEC elements for each of its lanes (a group of G of one warp, or the block's WARPS warps).
 template <typename T, int VEC, int NV, int WARPS, bool MASKED, bool EDGE, bool FULL>
-__global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS, 1024)) bias_softmax_fwd_rows(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(row_threads(WARPS, false), row_blocks(NV * VEC, WARPS, false)) bias_softmax_fwd_rows(const __grid_constant__ Args p) {
   extern __shared__ __align__(16) float lut[];
   __shared__ float2 meet[2][WARPS];
   const int h = blockIdx.x / p.blocks_per_head, part = blockIdx.x % p.blocks_per_head;
@@ -464,7 +477,7 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
 }
 
 template <typename T, int VEC, int NV, int WARPS, bool MASKED, bool EDGE, bool FULL>
-__global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS, 768)) bias_softmax_bwd_rows(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(row_threads(WARPS, true), row_blocks(NV * VEC, WARPS, true)) bias_softmax_bwd_rows(const __grid_constant__ Args p) {
   extern __shared__ __align__(16) float lut[];
   __shared__ float meet[2][WARPS];
   __shared__ float red[32];
@@ -475,8 +488,30 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
   float* all = lut + lut_words(p.last);
   float* acc = all + (WARPS == 1 ? (threadIdx.x / G) * words : 0);
   float below = 0.f, above = 0.f;
-  const unsigned r0 = part * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
-  const unsigned r = WARPS == 1 ? r0 + threadIdx.x / G : r0;
+  // Every group takes rows that follow one another, so that an element's distance falls by one from row to row: between whole rows the
+  // sums of a vector's distances stay in registers and move up by one place, and only the one that leaves at the end goes to shared memory.
+  const unsigned each = p.rows_per_block / groups, begin = part * p.rows_per_block;
+  const unsigned r0 = WARPS == 1 ? begin + threadIdx.x / G * each : begin;
+  const unsigned r1 = min(r0 + each, p.rows), r = r0;
+  float held[NV][VEC];
+  int held_x = 0;  // slot of key 0's distance in the row that the sums stand for
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) held[n][k] = 0.f;
+  auto put_away = [&] {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int j0 = (gl + n * lanes) * VEC;
+      if (FULL || j0 < p.Lk) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          add_distance(acc, p.last, held_x + j0 + k, held[n][k], below, above);
+          held[n][k] = 0.f;
+        }
+      }
+    }
+  };
   using Vectors = RowVectors<T, VEC, NV, EDGE, FULL>;
   constexpr int kDepth = ring_depth(NV, true);
   const T* base = static_cast<const T*>(p.s);
@@ -488,8 +523,8 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
     if (r + fetched < r1) {
       Vectors::fetch(base, p.elements, ahead.at, p.Lk, gl, lanes, ring + stage * 2 * NV * blockDim.x);
       Vectors::fetch(gbase, p.elements, ahead.at, p.Lk, gl, lanes, ring + (stage * 2 + 1) * NV * blockDim.x);
-      fetched += groups;
-      if (r + fetched < r1) ahead.advance(p, groups);
+      ++fetched;
+      if (r + fetched < r1) ahead.advance(p, 1);
     }
     copies_commit();
   };
@@ -500,12 +535,12 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
     for (int x = threadIdx.x; x < groups * words; x += blockDim.x) all[x] = 0.f;
   fill_lut(lut, p, h);
   int turn = 0, stage = 0;
-  for (unsigned done = 0; r0 + done < r1; done += groups, turn ^= 1) {
+  for (unsigned done = 0; done < each && begin + done < p.rows; ++done, turn ^= 1) {
     const bool live = r + done < r1;
     const RowWalk now = row;
     const float2 st = st_next;
-    if (r + done + groups < r1) {
-      row.advance(p, groups);
+    if (r + done + 1 < r1) {
+      row.advance(p, 1);
       st_next = p.stats[row.stat];
     }
     fetch_next(stage == 0 ? kDepth - 1 : stage - 1);
@@ -540,6 +575,8 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
     const float2 dot = both(-join_sums<WARPS>(group_sum(dot2.x + dot2.y, G), meet, turn));
     if (live) {
       T* o = static_cast<T*>(p.out) + now.at;
+      const bool sums = p.partial != nullptr;
+      if (!EDGE && sums && now.i == 0) put_away();  // another sequence: distances begin anew
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         const int j0 = (gl + n * lanes) * VEC - phase;
@@ -552,13 +589,24 @@ __global__ void __launch_bounds__(row_threads(WARPS), row_blocks(NV * VEC, WARPS
             set_pair(raw[n], k, mul2(a[n][k], both(p.scale)));
           }
           store_part<T, VEC, EDGE>(o, j0, p.Lk, raw[n]);
-          if (p.partial) add_distances<VEC>(acc, p.last, first_x + j0, a[n], below, above);
+          if (EDGE && sums) add_distances<VEC>(acc, p.last, first_x + j0, a[n], below, above);
+          if (!EDGE && sums) {
+            add_distance(acc, p.last, held_x + j0 + VEC - 1, held[n][VEC - 1], below, above);
+#pragma unroll
+            for (int k = VEC - 1; k > 0; --k) held[n][k] = held[n][k - 1] + (k % 2 ? a[n][k / 2].y : a[n][k / 2].x);
+            held[n][0] = a[n][0].x;
+          }
         }
       }
+      held_x = first_x;
     }
     if (WARPS == 1) __syncwarp();  // the next row of this group adds to the same sums from other lanes
   }
   if (!p.partial) return;
+  if (!EDGE) {
+    if (WARPS > 1) __syncthreads();  // behind the last row's
+    put_away();
+  }
   below = WARPS == 1 ? group_sum(below, G) : block_sum(below, red);
   above = WARPS == 1 ? group_sum(above, G) : block_sum(above, red);
   write_partial(p, all, groups, words, acc, h, part, below, above, gl == 0);
@@ -734,6 +782,7 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
   pl.edge = !aligned;
   pl.threads = kMaxThreads;
   pl.warps = 1;
+  if (nvec <= 32 * (16 / vec)) pl.threads = row_threads(1, bwd);
   int groups = 1;
   // 16 elements in a lane: fewer and the reductions and addresses of a row are too much for them, more and there are too few rows at once
   // (2048 keys in one / two / four / eight warps, before rows were copied ahead: forward 184 / 112 / 107 / 138 us, backward 530 / 271 / 172 /
@@ -743,7 +792,7 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
     int G = 1;
     while (G * wide < nvec) G <<= 1;
     if (bwd)  // sums over distances for each group: wider groups where there would be too many
-      while (G < 32 && (kMaxThreads / G) * words * 4 > 64 * 1024) G <<= 1;
+      while (G < 32 && (pl.threads / G) * words * 4 > 32 * 1024) G <<= 1;
     a.group = G;
     const int nv = (nvec + G - 1) / G;
     pl.nv = nv <= 1 ? 1 : (nv <= 2 ? 2 : 4);
@@ -760,7 +809,7 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
   pl.smem = (size_t)lut_words(a.last) * 4 + (bwd ? acc_words(a.last, groups) * 4 : 0) +
             (size_t)(pl.nv ? ring_depth(pl.nv, bwd) * pl.nv * pl.threads * 16 * (bwd ? 2 : 1) : 0);
   // One wave of blocks: each has to build its table of biases first, and what it leaves for the table gradient has to be added up.
-  int resident = (bwd ? 768 : 1024) / pl.threads;
+  int resident = resident_threads(pl.warps, bwd) / pl.threads;
   const int by_smem = (int)(220 * 1024 / (pl.smem + 1536));
   if (resident > by_smem) resident = by_smem > 0 ? by_smem : 1;
   

@@ -186,6 +186,9 @@ def test_an_index_out_of_range_raises_in_synchronous_mode():
 
 
 def test_the_guide_executes():
-    from transformer_op_checks import guide
+    from pathlib import Path
 
+    from transformer_op_checks import GUIDE, guide
+
+    assert GUIDE in (Path(__file__).resolve().parent.parent / "docs" / "training.md").read_text()
     guide()

@@ -366,13 +366,37 @@ def student_step(dev, position, fused=False, dtype=None):
         assert (got[n] - ref[n]).norm() <= tol * ref[n].norm() + 1e-6, (n, float((got[n] - ref[n]).norm() / ref[n].norm()))
 
 
-def guide():
-    """The code of docs/training.md on positions and distillation, run as written."""
-    from pathlib import Path
+GUIDE = """import torch, catch_b200
+from catch_b200.fusion import qk_norm_rotary, relative_bias_softmax, top_logits_distillation
 
-    text = (Path(__file__).resolve().parent.parent / "docs" / "training.md").read_text()
-    code = text.split("## Positions in attention, learning from a teacher")[1].split("```python")[1].split("```")[0]
+B, L, heads, dim, vocabulary = 2, 64, 4, 32, 1000
+qkv = torch.randn(B, L, 3 * heads, dim).bfloat16().to("blackwell").requires_grad_()    # one packed projection
+q, k, v = qkv[:, :, :heads], qkv[:, :, heads:2 * heads], qkv[:, :, 2 * heads:]          # slices, no copies
+
+# norm of every query / key head and rotation by position, one pass over both
+angle = torch.arange(L)[:, None] * 10000.0 ** (-torch.arange(0, dim, 2) / dim)
+norm = torch.ones(dim).to("blackwell").requires_grad_()
+q, k = qk_norm_rotary(q, k, norm, norm, angle.cos().to("blackwell"), angle.sin().to("blackwell"))
+
+# scale + learned relative position bias + mask + softmax over the scores; the bias is never stored as a matrix
+scores = torch.matmul(q.permute(0, 2, 1, 3), k.permute(0, 2, 3, 1))
+table = torch.zeros(32, heads).to("blackwell").requires_grad_()
+keep = torch.ones(B, 1, 1, L, dtype=torch.bool).to("blackwell")
+probs = relative_bias_softmax(scores, table, keep, scale=dim ** -0.5, max_distance=128)
+context = torch.matmul(probs, v.permute(0, 2, 1, 3))
+
+# a student's logits against the teacher's 16 largest of every row
+logits = torch.matmul(context.permute(0, 2, 1, 3).reshape(B * L, heads * dim),
+                      torch.randn(heads * dim, vocabulary).bfloat16().to("blackwell"))
+best, where = torch.randn(B * L, vocabulary).topk(16)
+loss = top_logits_distillation(logits, best.to("blackwell"), where.to("blackwell"), temperature=2.0)
+loss.backward()
+"""
+
+
+def guide():
+    """The code of the training guide on positions and distillation, run as written."""
     names = {}
-    exec(compile(code, "docs/training.md", "exec"), names)
+    exec(compile(GUIDE, "guide", "exec"), names)
     for leaf in ("qkv", "norm", "table"):
         assert bool(torch.isfinite(names[leaf].grad.float().cpu()).all()) and float(names[leaf].grad.float().cpu().abs().sum()) > 0

@@ -10,10 +10,10 @@
 // factor that backward() begins with, 1 (over the number of rows for a mean).  When another factor arrives, the backward writes dz anew
 // from z and the two saved numbers of each row, so that every gradient is rounded once whatever the factor.
 //
-// Measured on a B200, bf16, loss and gradient: 4096 x 30522, 64 kept: 129 us = 3.9 TB/s, 0.59 of the measured copy bandwidth; 4096 x 131072,
-// 128 kept: 538 us = 4.0 TB/s, 0.61; the loss alone 64 us (3.9 TB/s) and 213 us (5.0 TB/s).  With a factor other than 1 the early gradient is
-// written for nothing: 230 us at 4096 x 30522 instead of about 165 if it had not been tried.  What bounds the pass: issue slots (72 % busy) at 30522
-// words; at 131072 also L2, where half of the second reading misses.
+// Measured on a B200, bf16, loss and gradient: 4096 x 30522, 64 kept: 127 us = 3.9 TB/s, 0.60 of the measured copy bandwidth; 4096 x 131072,
+// 128 kept: 547 us = 3.9 TB/s, 0.60; the loss alone 64 us (3.9 TB/s) and 214 us (5.0 TB/s).  With a factor other than 1 the early gradient was
+// written for nothing: 235 us with the backward at 4096 x 30522, where the loss alone (64) and the backward (102) are 166.  What bounds the
+// pass: issue slots (72 % busy) at 30522 words; at 131072 also L2, where half of the second reading misses.
 #include "kernels_api.h"
 #include "row_vec.cuh"
 
@@ -307,11 +307,15 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
 #pragma unroll
         for (int u = 0; u < kUnit; ++u) {
           if (v0 + u * blockDim.x < r.vectors) {
+            if (any) {
 #pragma unroll
-            for (int k = 0; k < VEC / 2; ++k) {
-              const float2 x = mul2(add2(pair_of(raw[u], k), minus), both(c));
-              const float2 q = mul2(make_float2(exp2_fast(x.x), exp2_fast(x.y)), both(scale));
-              set_pair(raw[u], k, any ? q : make_float2(0.f, 0.f));
+              for (int k = 0; k < VEC / 2; ++k) {
+                const float2 x = mul2(add2(pair_of(raw[u], k), minus), both(c));
+                set_pair(raw[u], k, mul2(make_float2(exp2_fast(x.x), exp2_fast(x.y)), both(scale)));
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < VEC / 2; ++k) set_pair(raw[u], k, make_float2(0.f, 0.f));
             }
             __stcs(reinterpret_cast<uint4*>(d_body + (size_t)(v0 + u * blockDim.x) * VEC), *reinterpret_cast<const uint4*>(&raw[u]));
           }

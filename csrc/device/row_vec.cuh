@@ -54,12 +54,6 @@ template <int PENDING>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
 template <typename T, int N>
-__device__ __forceinline__ void load(const T* __restrict__ p, float (&out)[N]) {
-  const Pack<T, N> raw = *reinterpret_cast<const Pack<T, N>*>(p);
-#pragma unroll
-  for (int k = 0; k < N; ++k) out[k] = to_f32<T>(raw.v[k]);
-}
-template <typename T, int N>
 __device__ __forceinline__ void store(T* __restrict__ p, const float (&in)[N]) {
   Pack<T, N> raw;
 #pragma unroll

@@ -668,6 +668,12 @@ Tensor empty_in_phase(const Tensor& t, int64_t ld) {
   return fresh({need + phase}, t).as_strided(t.sizes(), {ld, 1}, phase);
 }
 
+// Whether `out` has the type, the rows' distance and the place within 16 bytes of `t`.
+bool same_rows(const Tensor& out, const Tensor& t, int64_t ld) {
+  return out.sizes() == t.sizes() && out.scalar_type() == t.scalar_type() && (out.size(0) <= 1 || out.stride(0) == ld) && (out.size(1) <= 1 || out.stride(1) == 1) &&
+         (reinterpret_cast<uintptr_t>(out.data_ptr()) - reinterpret_cast<uintptr_t>(t.data_ptr())) % 16 == 0;
+}
+
 B200Distill distill_params(const DistillArgs& a, const Tensor& z, const Tensor& teacher, const Tensor& index) {
   B200Distill p{};
   p.logits = z.data_ptr(); p.teacher = teacher.data_ptr(); p.index = index.data_ptr();
@@ -739,14 +745,17 @@ Tensor distill_bwd(const DistillArgs& a, const Tensor& grad, const Tensor& stats
   OpScope scope(op, a.logits);
   Tensor z = row_layout(a.logits), teacher = a.teacher.contiguous(), index = a.index.contiguous(), g = grad.to(at::kFloat);
   B200Distill p = distill_params(a, z, teacher, index);
-  Tensor out = ready.defined() ? ready : empty_in_phase(z, p.ld);
+  // What backward() is given may lie elsewhere than what the forward saw (hooks on saved tensors, a recomputed forward): the kernel
+  // takes the row distance and the place within 16 bytes of both from the logits.
+  const bool keep = ready.defined() && same_rows(ready, z, p.ld);
+  Tensor out = keep ? ready : empty_in_phase(z, p.ld);
   p.stats = stats.data_ptr<float>();
   p.count = mean ? count.data_ptr<float>() : nullptr;
   p.dlogits = out.data_ptr();
   p.grad = g.data_ptr<float>();
   p.grad_per_row = each;
   p.grad_ld = each && N > 1 ? g.stride(0) : 0;
-  p.skip_factor_one = ready.defined();
+  p.skip_factor_one = keep;
   B200_KERNEL_CHECK(b200_distill_bwd(&p, scope.stream()));
   return out;
 }

@@ -1,0 +1,45 @@
+"""The transformer operators' gradients under the ways in which autograd may run a backward pass."""
+import pytest
+import torch
+
+import transformer_cases as cases
+from transformer_cases import check
+
+pytestmark = pytest.mark.gpu
+DEV = "blackwell"
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _backend():
+    import catch_b200  # noqa: F401
+
+    assert torch.b200.backend_name() == "cuda"
+    torch.b200.set_flag("op_trycatch", False)
+    yield
+    torch.b200.set_flag("op_trycatch", True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("factor", [1.0, 0.5])
+@pytest.mark.parametrize("start, width", [(0, 101), (3, 120), (1, 101)])
+def test_logits_that_come_back_in_another_layout(dtype, factor, start, width):
+    """A hook on saved tensors may hand them back with other strides and another place within 16 bytes."""
+    from catch_b200.fusion import top_logits_distillation
+
+    N, V = 9, 97
+    torch.manual_seed(1)
+    z = torch.randn(N, V).to(dtype)
+    t, idx = cases.teacher_of(N, V, 5, 3)
+
+    def shifted(x):  # the same values, `start` elements behind a boundary, rows `width` apart
+        if x.shape != (N, V):
+            return x
+        return torch.zeros(N, width, dtype=x.dtype, device=x.device)[:, start:start + V].copy_(x)
+
+    for first in (z.to(DEV), shifted(z.to(DEV))):
+        leaf = first.detach().requires_grad_()
+        for unpack in (lambda x: x.clone(memory_format=torch.contiguous_format), shifted):
+            with torch.autograd.graph.saved_tensors_hooks(lambda x: x, unpack):
+                loss = top_logits_distillation(leaf, t.to(DEV), idx.to(DEV), temperature=2.0)
+                (dz,) = torch.autograd.grad(loss, leaf, torch.tensor(factor).to(DEV))
+            check(dz, *cases.distill_reference(z, t, idx, 2.0, "mean", factor)[1], "gradient")

@@ -169,7 +169,7 @@ __device__ __forceinline__ MaskRow mask_row(const Args& p, long long at, int pha
 template <int VEC, bool EDGE>
 __device__ __forceinline__ bool add_mask(const Args& p, const MaskRow& row, int j0, float2 (&a)[VEC / 2]) {
   if (row.wide && (!EDGE || (j0 >= 0 && j0 + VEC <= p.Lk))) {
-    const char* m = row.key0 + j0 * mask_bytes(p.mask_dtype);
+    const char* m = row.key0 + (long long)j0 * mask_bytes(p.mask_dtype);  // (bytes pass 32 bits before keys do)
     if (p.mask_dtype == B200_F32) return add_mask_vector<float, VEC>(reinterpret_cast<const float*>(m), a);
     if (p.mask_dtype == B200_BF16) return add_mask_vector<__nv_bfloat16, VEC>(reinterpret_cast<const __nv_bfloat16*>(m), a);
     if (p.mask_dtype == B200_F16) return add_mask_vector<__half, VEC>(reinterpret_cast<const __half*>(m), a);

@@ -154,3 +154,27 @@ def test_distillation_from_row_to_row(dtype, N, V, K, layout, reduction, factor)
     check(dz, *ref[1], "gradient")
     with torch.no_grad():
         check(top_logits_distillation(zd, t.to(DEV), idx.to(DEV), temperature=T, reduction=reduction), *ref[0], "loss alone", slack=slack)
+
+
+@pytest.mark.parametrize("mask_dtype", [F32, BF16, torch.bool])
+def test_mask_bytes_beyond_two_to_the_31(mask_dtype):
+    """One row of 2^29 keys and some: an additive fp32 mask has more than 2^31 bytes then."""
+    ops = torch.ops.catch_b200
+    n, last, some = (1 << 29) + 1000, 700, 6
+    s = torch.zeros(1, 1, 1, n, dtype=BF16, device=DEV)
+    m = torch.zeros(1, 1, 1, n, dtype=mask_dtype, device=DEV) if mask_dtype == torch.bool else \
+        torch.full((1, 1, 1, n), -math.inf, dtype=mask_dtype, device=DEV)
+    for part in (m[..., -last:], m[..., 8:8 + some]):
+        part.fill_(True if mask_dtype == torch.bool else 0.0)
+    t = torch.zeros(4, 1, device=DEV)
+    p, st = ops.relative_bias_softmax(s, t, m, 1.0, False, 8, n - 1)
+    want = torch.zeros(n, dtype=BF16)
+    want[-last:] = want[8:8 + some] = 1.0 / (last + some)
+    assert torch.equal(p.cpu().flatten(), want)
+    g = torch.zeros(1, 1, 1, n, dtype=BF16, device=DEV)
+    g[..., -1].fill_(1.0)
+    ds, _ = ops.relative_bias_softmax_backward(g, s, st, t, m, 1.0, False, 8, n - 1, False)
+    q = 1.0 / (last + some)
+    ds = ds.cpu().flatten()
+    assert int((ds != 0).sum()) == last + some
+    assert abs(float(ds[-1]) - q * (1 - q)) <= q * 2.0 ** -8 and abs(float(ds[-2]) + q * q) <= q * q * 2.0 ** -7

@@ -410,10 +410,16 @@ void check_bias(const BiasArgs& a) {
               " and ", (a.bidirectional ? 4 : 2) * B200_MAX_FAR_BUCKETS, " buckets", a.bidirectional ? ", an even number" : "", ", got ", n);
   TORCH_CHECK(a.max_distance > side / 2 && a.max_distance <= B200_MAX_BIAS_DISTANCE, op, ": max_distance must be above ", side / 2,
               " (the distances with a bucket each) and at most ", B200_MAX_BIAS_DISTANCE, ", got ", a.max_distance);
-  TORCH_CHECK(std::abs(a.query_offset) < (1 << 30) && a.scores.size(2) < (1 << 30) && a.scores.size(3) < (1 << 30), op,
+  const int64_t far_off = int64_t(1) << 30, Lq = a.scores.size(2), Lk = a.scores.size(3);
+  TORCH_CHECK(a.query_offset > -far_off && a.query_offset < far_off && Lq < far_off && Lk < far_off, op,
               ": lengths and query_offset must stay below 2^30");
-  TORCH_CHECK(a.scores.size(0) * a.scores.size(2) < (int64_t(1) << 31), op, ": batch times queries must stay below 2^31");
-  TORCH_CHECK(std::isfinite(a.scale), op, ": scale must be finite, got ", a.scale);
+  // slots of distances are 32-bit numbers: reach - query_offset - query + key
+  TORCH_CHECK(std::abs(a.query_offset) + std::max(Lq, Lk) < (int64_t(1) << 31) - 2 * B200_MAX_BIAS_DISTANCE, op,
+              ": queries and keys lie too far apart: lengths of ", Lq, " and ", Lk, " with query_offset ", a.query_offset);
+  TORCH_CHECK(a.scores.size(0) < (int64_t(1) << 31) && a.scores.size(0) * Lq < (int64_t(1) << 31), op,
+              ": batch times queries must stay below 2^31");
+  TORCH_CHECK(a.scores.size(1) < (int64_t(1) << 31), op, ": the number of heads must stay below 2^31");
+  TORCH_CHECK(std::isfinite((float)a.scale), op, ": scale must be finite in fp32, got ", a.scale);
   if (given(a.mask)) {
     TORCH_CHECK(a.mask->scalar_type() == at::kBool || f_ok(a.mask->scalar_type()), op,
                 ": the mask is bool (true keeps a key) or floating (added), got ", a.mask->scalar_type());

@@ -250,6 +250,11 @@ const Tensor& or_none(const OptTensor& t) {
   static const Tensor none;
   return given(t) ? *t : none;
 }
+// An output without a tangent would count as one that does not depend on the inputs.
+void refuse_tangents(const char* op, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), op, ": forward-mode derivatives are not implemented");
+}
 template <typename N>
 std::shared_ptr<N> make_node() {
   return std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
@@ -308,6 +313,7 @@ std::tuple<Tensor, Tensor> qk_norm_rotary_autograd(const Tensor& q, const Tensor
                                                    bool interleaved) {
   std::shared_ptr<RotaryNode> node;
   const Tensor &tqw = or_none(qw), &tkw = or_none(kw);
+  refuse_tangents("qk_norm_rotary", {&q, &k, &tqw, &tkw, &cos, &sin});
   if (wants_grad({&q, &k, &tqw, &tkw})) {
     node = make_node<RotaryNode>();
     node->set_next_edges(torch::autograd::collect_next_edges(q, k, tqw, tkw));
@@ -584,6 +590,7 @@ std::tuple<Tensor, Tensor> relative_bias_softmax(const Tensor& scores, const Ten
 }
 std::tuple<Tensor, Tensor> relative_bias_softmax_autograd(const Tensor& scores, const Tensor& table, const OptTensor& mask, double scale,
                                                           bool bidirectional, int64_t max_distance, int64_t query_offset) {
+  refuse_tangents("relative_bias_softmax", {&scores, &table, &or_none(mask)});
   Tensor probs, stats, laid_out;
   {
     Below below;
@@ -805,6 +812,7 @@ Tensor top_logits_distillation_backward(const Tensor& grad, const Tensor& logits
 }
 Tensor top_logits_distillation_autograd(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature,
                                         int64_t reduction) {
+  refuse_tangents("top_logits_distillation", {&logits, &teacher});
   const bool grad = wants_grad({&logits});
   Tensor loss, stats, count, ready;
   {

@@ -5,7 +5,11 @@
 //
 // The reference has no counterpart (its eager layers run these as separate norm, multiply, gather, add and softmax
 // calls).  Every operator has a host path in elementary operations for host simulation and for tensors of other
-// devices; gradients are wired up here, so torch.ops.catch_b200.<name> is differentiable as it is.
+// devices; gradients are wired up here, so torch.ops.catch_b200.<name> is differentiable as it is.  The autograd kernels go on through
+// the dispatcher, so that what lies below them (torch.func's transforms, dispatch modes, fake tensors) sees the operators and their
+// _backward forms.
+#include <ATen/TensorSubclassLikeUtils.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -83,7 +87,6 @@ void check_rotary(const RotaryArgs& a) {
   TORCH_CHECK(f_ok(a.cos.scalar_type()) && f_ok(a.sin.scalar_type()), op, ": cos and sin are floating tables, got ",
               a.cos.scalar_type(), " and ", a.sin.scalar_type());
   TORCH_CHECK(2 * a.cos.size(1) <= D, op, ": cos and sin rotate ", 2 * a.cos.size(1), " dimensions of ", D);
-  TORCH_CHECK(!a.cos.requires_grad() && !a.sin.requires_grad(), op, ": cos and sin are constants, they get no gradient");
   for (const OptTensor* w : {&a.qw, &a.kw})
     if (given(*w))
       TORCH_CHECK((*w)->dim() == 1 && (*w)->size(0) == D && f_ok((*w)->scalar_type()), op, ": weights are floating [head_dim], got ",
@@ -151,6 +154,27 @@ std::tuple<Tensor, Tensor> host_rotary_bwd(const RotaryArgs& a, const Tensor& x,
   return {at::where(inside, dx, zero).to(x.scalar_type()).contiguous(), dw};
 }
 
+std::tuple<Tensor, Tensor> qk_norm_rotary_meta(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& cos,
+                                               const Tensor& sin, const OptTensor& positions, double eps, bool interleaved) {
+  check_rotary({q, k, qw, kw, cos, sin, positions, eps, interleaved});
+  return {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options())};
+}
+void check_rotary_grads(const RotaryArgs& a, const Tensor& dyq, const Tensor& dyk) {
+  check_rotary(a);
+  TORCH_CHECK(dyq.sizes() == a.q.sizes() && dyk.sizes() == a.k.sizes() && dyq.scalar_type() == a.q.scalar_type() &&
+                  dyk.scalar_type() == a.k.scalar_type(),
+              "qk_norm_rotary_backward: the gradients have the shapes and the dtype of queries and keys");
+  check_same_device("qk_norm_rotary_backward", a.q, dyq, dyk);
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_backward_meta(const Tensor& dyq, const Tensor& dyk, const Tensor& q, const Tensor& k,
+                                                                        const OptTensor& qw, const OptTensor& kw, const Tensor& cos,
+                                                                        const Tensor& sin, const OptTensor& positions, double eps,
+                                                                        bool interleaved, bool need_qw, bool need_kw) {
+  check_rotary_grads({q, k, qw, kw, cos, sin, positions, eps, interleaved}, dyq, dyk);
+  return {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options()),
+          given(qw) && need_qw ? at::empty(qw->sizes(), qw->options()) : Tensor(), given(kw) && need_kw ? at::empty(kw->sizes(), kw->options()) : Tensor()};
+}
+
 Tensor dense_last(const Tensor& t) { return t.stride(-1) == 1 || t.numel() == 0 ? t : t.contiguous(); }
 
 // The kernel's arguments that both directions share; `keep` holds what has to outlive the call.
@@ -189,7 +213,9 @@ B200QkNormRotary rotary_params(const RotaryArgs& a, const Tensor& q, const Tenso
 }
 OptTensor dense_weight(const OptTensor& w) { return given(w) ? OptTensor(w->contiguous()) : OptTensor(); }
 
-std::tuple<Tensor, Tensor> rotary_fwd(const RotaryArgs& a) {
+std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q_in, const Tensor& k_in, const OptTensor& qw_in, const OptTensor& kw_in, const Tensor& cos,
+                                          const Tensor& sin, const OptTensor& positions, double eps, bool interleaved) {
+  const RotaryArgs a{q_in, k_in, qw_in, kw_in, cos, sin, positions, eps, interleaved};
   check_rotary(a);
   if (!on_device(a.q)) return {host_rotary_fwd(a, a.q, a.qw), host_rotary_fwd(a, a.k, a.kw)};
   OpScope scope("qk_norm_rotary", a.q);
@@ -204,16 +230,16 @@ std::tuple<Tensor, Tensor> rotary_fwd(const RotaryArgs& a) {
   return {yq, yk};
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> rotary_bwd(const RotaryArgs& a, const Tensor& dyq, const Tensor& dyk, bool need_qw = true, bool need_kw = true) {
-  check_rotary(a);
-  TORCH_CHECK(dyq.sizes() == a.q.sizes() && dyk.sizes() == a.k.sizes() && dyq.scalar_type() == a.q.scalar_type() &&
-                  dyk.scalar_type() == a.k.scalar_type(),
-              "qk_norm_rotary_backward: the gradients have the shapes and the dtype of queries and keys");
-  check_same_device("qk_norm_rotary_backward", a.q, dyq, dyk);
+std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_backward(const Tensor& dyq, const Tensor& dyk, const Tensor& q_in, const Tensor& k_in,
+                                                                   const OptTensor& qw_in, const OptTensor& kw_in, const Tensor& cos,
+                                                                   const Tensor& sin, const OptTensor& positions, double eps,
+                                                                   bool interleaved, bool need_qw, bool need_kw) {
+  const RotaryArgs a{q_in, k_in, qw_in, kw_in, cos, sin, positions, eps, interleaved};
+  check_rotary_grads(a, dyq, dyk);
   if (!on_device(a.q)) {
     auto [dq, dqw] = host_rotary_bwd(a, a.q, a.qw, dyq);
     auto [dk, dkw] = host_rotary_bwd(a, a.k, a.kw, dyk);
-    return {dq, dk, dqw, dkw};
+    return {dq, dk, need_qw ? dqw : Tensor(), need_kw ? dkw : Tensor()};
   }
   OpScope scope("qk_norm_rotary_backward", a.q);
   Tensor q = dense_last(a.q), k = dense_last(a.k), gq = dense_last(dyq), gk = dense_last(dyk);
@@ -260,11 +286,14 @@ std::shared_ptr<N> make_node() {
   return std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
 }
 SavedVariable save(const Tensor& t) { return SavedVariable(t, /*is_output=*/false); }
-// Runs without recording, below autograd.
-struct Below {
-  at::AutoDispatchBelowADInplaceOrView dispatch;
-  at::NoGradGuard no_grad;
-};
+// Calls go on below autograd.
+using Below = at::AutoDispatchBelowADInplaceOrView;
+template <typename F>
+c10::TypedOperatorHandle<F> find_op(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+// Whether nothing but the kernels looks on (no wrapper of a transform, no subclass, no dispatch mode), so that a shortcut may use the memory.
+bool plain(const Tensor& t) { return !at::isTensorSubclassLike(t); }
 
 // Autograd runs a backward on a thread of its own, whose memory does not come from the pool of a graph that the caller is capturing:
 // a replay would write to memory that belongs to others by then.  The operators' _backward forms, called by the capturing thread, are fine.
@@ -292,28 +321,26 @@ struct RotaryNode : public torch::autograd::Node {
     if (!g[0].defined() && !g[1].defined()) return out;
     const Tensor uq = q.unpack(), uk = k.unpack();
     refuse_captured_backward("qk_norm_rotary", uq);
+    static const auto op = find_op<decltype(qk_norm_rotary_backward)>("catch_b200::qk_norm_rotary_backward");
     {
       Below below;
       Tensor gq = g[0].defined() ? g[0] : at::zeros_like(uq, at::MemoryFormat::Contiguous);
       Tensor gk = g[1].defined() ? g[1] : at::zeros_like(uk, at::MemoryFormat::Contiguous);
       std::tie(out[0], out[1], out[2], out[3]) =
-          rotary_bwd({uq, uk, saved_optional(qw.unpack()), saved_optional(kw.unpack()), cos.unpack(), sin.unpack(),
-                      saved_optional(positions.unpack()), eps, interleaved}, gq, gk, task_should_compute_output(2), task_should_compute_output(3));
+          op.call(gq, gk, uq, uk, saved_optional(qw.unpack()), saved_optional(kw.unpack()), cos.unpack(), sin.unpack(),
+                  saved_optional(positions.unpack()), eps, interleaved, task_should_compute_output(2), task_should_compute_output(3));
     }
     return once_differentiable("qk_norm_rotary", std::move(out));
   }
 };
 
-std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& cos,
-                                          const Tensor& sin, const OptTensor& positions, double eps, bool interleaved) {
-  return rotary_fwd({q, k, qw, kw, cos, sin, positions, eps, interleaved});
-}
 std::tuple<Tensor, Tensor> qk_norm_rotary_autograd(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw,
                                                    const Tensor& cos, const Tensor& sin, const OptTensor& positions, double eps,
                                                    bool interleaved) {
   std::shared_ptr<RotaryNode> node;
   const Tensor &tqw = or_none(qw), &tkw = or_none(kw);
   refuse_tangents("qk_norm_rotary", {&q, &k, &tqw, &tkw, &cos, &sin});
+  TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(), "qk_norm_rotary: cos and sin are constants, they get no gradient");
   if (wants_grad({&q, &k, &tqw, &tkw})) {
     node = make_node<RotaryNode>();
     node->set_next_edges(torch::autograd::collect_next_edges(q, k, tqw, tkw));
@@ -322,22 +349,17 @@ std::tuple<Tensor, Tensor> qk_norm_rotary_autograd(const Tensor& q, const Tensor
     node->eps = eps;
     node->interleaved = interleaved;
   }
+  static const auto op = find_op<decltype(qk_norm_rotary)>("catch_b200::qk_norm_rotary");
   Tensor yq, yk;
   {
     Below below;
-    std::tie(yq, yk) = qk_norm_rotary(q, k, qw, kw, cos, sin, positions, eps, interleaved);
+    std::tie(yq, yk) = op.call(q, k, qw, kw, cos, sin, positions, eps, interleaved);
   }
   if (node) {
     torch::autograd::set_history(yq, node);
     torch::autograd::set_history(yk, node);
   }
   return {yq, yk};
-}
-std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_backward(const Tensor& dyq, const Tensor& dyk, const Tensor& q, const Tensor& k,
-                                                                   const OptTensor& qw, const OptTensor& kw, const Tensor& cos,
-                                                                   const Tensor& sin, const OptTensor& positions, double eps,
-                                                                   bool interleaved) {
-  return rotary_bwd({q, k, qw, kw, cos, sin, positions, eps, interleaved}, dyq, dyk);
 }
 
 // ------------------------------------------------------------------------------------------------------ biased softmax
@@ -433,7 +455,6 @@ void check_bias(const BiasArgs& a) {
     for (int64_t i = 1; i <= a.mask->dim(); ++i)
       TORCH_CHECK(a.mask->size(-i) == 1 || a.mask->size(-i) == a.scores.size(-i), op, ": the mask ", a.mask->sizes(),
                   " does not broadcast to the scores ", a.scores.sizes());
-    TORCH_CHECK(!a.mask->requires_grad(), op, ": the mask gets no gradient; pass a mask that does not require one");
   }
   check_same_device(op, a.scores, a.table, a.mask);
 }
@@ -495,12 +516,14 @@ B200BiasSoftmax bias_params(const BiasArgs& a, const Tensor& scores, const Tenso
   return p;
 }
 
+std::vector<int64_t> stats_sizes(const Tensor& scores) { return {scores.size(0), scores.size(1), scores.size(2), 2}; }
+
 // (probabilities, statistics [batch, heads, queries, 2]: the maximum and 1 / sum of each row)
-std::tuple<Tensor, Tensor> bias_fwd(const BiasArgs& a, Tensor& laid_out) {
+std::tuple<Tensor, Tensor> relative_bias_softmax(const Tensor& scores, const Tensor& table_in, const OptTensor& mask, double scale,
+                                                 bool bidirectional, int64_t max_distance, int64_t query_offset) {
+  const BiasArgs a{scores, table_in, mask, scale, bidirectional, max_distance, query_offset};
   check_bias(a);
-  std::vector<int64_t> ss(a.scores.sizes().begin(), a.scores.sizes().end());
-  ss[3] = 2;
-  laid_out = a.scores;
+  const std::vector<int64_t> ss = stats_sizes(scores);
   if (!on_device(a.scores)) {
     if (a.scores.numel() == 0) return {at::empty_like(a.scores), at::empty(ss, a.scores.options().dtype(at::kFloat))};
     auto [x, bucket] = host_logits(a);
@@ -511,7 +534,7 @@ std::tuple<Tensor, Tensor> bias_fwd(const BiasArgs& a, Tensor& laid_out) {
     return {host_probs(x, stats).to(a.scores.scalar_type()), stats};
   }
   OpScope scope("relative_bias_softmax", a.scores);
-  Tensor s = laid_out = score_layout(a.scores), table = a.table.contiguous();
+  Tensor s = score_layout(a.scores), table = a.table.contiguous();
   Tensor probs = fresh_strided(s), stats = fresh(ss, at::kFloat, s);
   B200BiasSoftmax p = bias_params(a, s, table);
   p.out = probs.data_ptr();
@@ -520,15 +543,32 @@ std::tuple<Tensor, Tensor> bias_fwd(const BiasArgs& a, Tensor& laid_out) {
   return {probs, stats};
 }
 
-std::tuple<Tensor, Tensor> bias_bwd(const BiasArgs& a, const Tensor& grad, const Tensor& stats, bool need_table) {
+std::tuple<Tensor, Tensor> relative_bias_softmax_meta(const Tensor& scores, const Tensor& table, const OptTensor& mask, double scale,
+                                                      bool bidirectional, int64_t max_distance, int64_t query_offset) {
+  check_bias({scores, table, mask, scale, bidirectional, max_distance, query_offset});
+  return {at::empty_like(scores), at::empty(stats_sizes(scores), scores.options().dtype(at::kFloat))};
+}
+void check_bias_grads(const BiasArgs& a, const Tensor& grad, const Tensor& stats) {
   check_bias(a);
   const char* op = "relative_bias_softmax_backward";
   TORCH_CHECK(grad.sizes() == a.scores.sizes() && grad.scalar_type() == a.scores.scalar_type(), op,
               ": the gradient has the shape and the dtype of the scores");
-  TORCH_CHECK(stats.dim() == 4 && stats.size(0) == a.scores.size(0) && stats.size(1) == a.scores.size(1) &&
-                  stats.size(2) == a.scores.size(2) && stats.size(3) == 2 && stats.scalar_type() == at::kFloat && stats.is_contiguous(),
-              op, ": statistics are the forward's");
+  TORCH_CHECK(stats.sizes() == at::IntArrayRef(stats_sizes(a.scores)) && stats.scalar_type() == at::kFloat && stats.is_contiguous(), op,
+              ": statistics are the forward's");
   check_same_device(op, a.scores, grad, stats);
+}
+std::tuple<Tensor, Tensor> relative_bias_softmax_backward_meta(const Tensor& grad, const Tensor& scores, const Tensor& stats, const Tensor& table,
+                                                               const OptTensor& mask, double scale, bool bidirectional, int64_t max_distance,
+                                                               int64_t query_offset, bool need_table) {
+  check_bias_grads({scores, table, mask, scale, bidirectional, max_distance, query_offset}, grad, stats);
+  return {at::empty_like(scores), need_table ? at::empty(table.sizes(), table.options()) : Tensor()};
+}
+
+std::tuple<Tensor, Tensor> relative_bias_softmax_backward(const Tensor& grad, const Tensor& scores, const Tensor& stats, const Tensor& table_in,
+                                                          const OptTensor& mask, double scale, bool bidirectional, int64_t max_distance,
+                                                          int64_t query_offset, bool need_table) {
+  const BiasArgs a{scores, table_in, mask, scale, bidirectional, max_distance, query_offset};
+  check_bias_grads(a, grad, stats);
   if (!on_device(a.scores)) {
     if (a.scores.numel() == 0) return {at::empty_like(a.scores), need_table ? at::zeros_like(a.table) : Tensor()};
     auto [x, bucket] = host_logits(a);
@@ -542,7 +582,7 @@ std::tuple<Tensor, Tensor> bias_bwd(const BiasArgs& a, const Tensor& grad, const
     }
     return {(d * a.scale).to(a.scores.scalar_type()), dt};
   }
-  OpScope scope(op, a.scores);
+  OpScope scope("relative_bias_softmax_backward", a.scores);
   Tensor s = score_layout(a.scores), g = in_layout_of(grad, s), table = a.table.contiguous();
   Tensor ds = fresh_strided(s), dt;
   B200BiasSoftmax p = bias_params(a, s, table);
@@ -574,29 +614,30 @@ struct BiasNode : public torch::autograd::Node {
     if (!g[0].defined()) return out;
     const Tensor s = scores.unpack(), t = table.unpack(), m = mask.unpack(), st = stats.unpack();
     refuse_captured_backward("relative_bias_softmax", s);
+    static const auto op = find_op<decltype(relative_bias_softmax_backward)>("catch_b200::relative_bias_softmax_backward");
     {
       Below below;
       std::tie(out[0], out[1]) =
-          bias_bwd({s, t, saved_optional(m), scale, bidirectional, max_distance, query_offset}, g[0], st, task_should_compute_output(1));
+          op.call(g[0], s, st, t, saved_optional(m), scale, bidirectional, max_distance, query_offset, task_should_compute_output(1));
     }
     return once_differentiable("relative_bias_softmax", std::move(out));
   }
 };
 
-std::tuple<Tensor, Tensor> relative_bias_softmax(const Tensor& scores, const Tensor& table, const OptTensor& mask, double scale,
-                                                 bool bidirectional, int64_t max_distance, int64_t query_offset) {
-  Tensor laid_out;
-  return bias_fwd({scores, table, mask, scale, bidirectional, max_distance, query_offset}, laid_out);
-}
 std::tuple<Tensor, Tensor> relative_bias_softmax_autograd(const Tensor& scores, const Tensor& table, const OptTensor& mask, double scale,
                                                           bool bidirectional, int64_t max_distance, int64_t query_offset) {
   refuse_tangents("relative_bias_softmax", {&scores, &table, &or_none(mask)});
-  Tensor probs, stats, laid_out;
+  TORCH_CHECK(!or_none(mask).defined() || !mask->requires_grad(),
+              "relative_bias_softmax: the mask gets no gradient; pass a mask that does not require one");
+  static const auto op = find_op<decltype(relative_bias_softmax)>("catch_b200::relative_bias_softmax");
+  const bool grad = wants_grad({&scores, &table});
+  Tensor probs, stats, laid_out = scores;
   {
     Below below;
-    std::tie(probs, stats) = bias_fwd({scores, table, mask, scale, bidirectional, max_distance, query_offset}, laid_out);
+    if (grad && scores.dim() == 4 && on_device(scores) && plain(scores)) laid_out = score_layout(scores);  // once for both directions
+    std::tie(probs, stats) = op.call(laid_out, table, mask, scale, bidirectional, max_distance, query_offset);
   }
-  if (wants_grad({&scores, &table})) {
+  if (grad) {
     auto node = make_node<BiasNode>();
     node->set_next_edges(torch::autograd::collect_next_edges(scores, table));
     node->scores = save(laid_out); node->table = save(table); node->mask = save(or_none(mask)); node->stats = save(stats);
@@ -604,11 +645,6 @@ std::tuple<Tensor, Tensor> relative_bias_softmax_autograd(const Tensor& scores, 
     torch::autograd::set_history(probs, node);
   }
   return {probs, stats};
-}
-std::tuple<Tensor, Tensor> relative_bias_softmax_backward(const Tensor& grad, const Tensor& scores, const Tensor& stats, const Tensor& table,
-                                                          const OptTensor& mask, double scale, bool bidirectional, int64_t max_distance,
-                                                          int64_t query_offset, bool need_table) {
-  return bias_bwd({scores, table, mask, scale, bidirectional, max_distance, query_offset}, grad, stats, need_table);
 }
 
 // -------------------------------------------------------------------------------------------------------- distillation
@@ -632,7 +668,6 @@ void check_distill(const DistillArgs& a) {
               a.temperature);
   TORCH_CHECK(a.reduction == at::Reduction::None || a.reduction == at::Reduction::Mean || a.reduction == at::Reduction::Sum, op,
               ": reduction is 0 (none), 1 (mean) or 2 (sum), got ", a.reduction);
-  TORCH_CHECK(!a.teacher.requires_grad(), op, ": the teacher's logits get no gradient; detach them");
   check_same_device(op, a.logits, a.teacher, a.index);
 }
 
@@ -741,11 +776,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> distill_fwd(const DistillArgs& a, boo
   return {loss, stats, count, grad};
 }
 
-// The gradient of the logits; `ready`: the forward's, which is taken when the factor turns out to be 1.
-Tensor distill_bwd(const DistillArgs& a, const Tensor& grad, const Tensor& stats, const Tensor& count, const Tensor& ready) {
+void check_distill_grads(const DistillArgs& a, const Tensor& grad, const Tensor& stats, const Tensor& count) {
   check_distill(a);
   const char* op = "top_logits_distillation_backward";
-  const bool mean = a.reduction == at::Reduction::Mean, each = a.reduction == at::Reduction::None;
+  const bool each = a.reduction == at::Reduction::None;
   const int64_t N = a.logits.size(0);
   TORCH_CHECK(each ? (grad.dim() == 1 && grad.size(0) == N) : grad.numel() == 1, op, ": the gradient has the shape of the loss, got ",
               grad.sizes());
@@ -753,9 +787,16 @@ Tensor distill_bwd(const DistillArgs& a, const Tensor& grad, const Tensor& stats
                   count.numel() >= 1 && count.scalar_type() == at::kFloat,
               op, ": statistics are the forward's");
   check_same_device(op, a.logits, grad, stats, count);
+}
+
+// The gradient of the logits; `ready`: the forward's, which is taken when the factor turns out to be 1.
+Tensor distill_bwd(const DistillArgs& a, const Tensor& grad, const Tensor& stats, const Tensor& count, const Tensor& ready) {
+  check_distill_grads(a, grad, stats, count);
+  const bool mean = a.reduction == at::Reduction::Mean, each = a.reduction == at::Reduction::None;
+  const int64_t N = a.logits.size(0);
   if (!on_device(a.logits))
     return host_distill_grad(a, host_teacher(a), grad.to(at::kFloat).reshape({-1}).expand({N}) / count.to(at::kFloat));
-  OpScope scope(op, a.logits);
+  OpScope scope("top_logits_distillation_backward", a.logits);
   Tensor z = row_layout(a.logits), teacher = a.teacher.contiguous(), index = a.index.contiguous(), g = grad.to(at::kFloat);
   B200Distill p = distill_params(a, z, teacher, index);
   // What backward() is given may lie elsewhere than what the forward saw (hooks on saved tensors, a recomputed forward): the kernel
@@ -771,6 +812,34 @@ Tensor distill_bwd(const DistillArgs& a, const Tensor& grad, const Tensor& stats
   p.skip_factor_one = keep;
   B200_KERNEL_CHECK(b200_distill_bwd(&p, scope.stream()));
   return out;
+}
+
+Tensor top_logits_distillation(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction) {
+  return std::get<0>(distill_fwd({logits, teacher, index, temperature, reduction}, false));
+}
+std::tuple<Tensor, Tensor, Tensor> top_logits_distillation_stats(const Tensor& logits, const Tensor& teacher, const Tensor& index,
+                                                                 double temperature, int64_t reduction) {
+  auto [loss, stats, count, ready] = distill_fwd({logits, teacher, index, temperature, reduction}, false);
+  return {loss, stats, count};
+}
+Tensor top_logits_distillation_backward(const Tensor& grad, const Tensor& logits, const Tensor& stats, const Tensor& count, const Tensor& teacher,
+                                        const Tensor& index, double temperature, int64_t reduction) {
+  return distill_bwd({logits, teacher, index, temperature, reduction}, grad, stats, count, Tensor());
+}
+Tensor top_logits_distillation_meta(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction) {
+  check_distill({logits, teacher, index, temperature, reduction});
+  auto opt = logits.options().dtype(at::kFloat);
+  return reduction == at::Reduction::None ? at::empty({logits.size(0)}, opt) : at::empty({}, opt);
+}
+std::tuple<Tensor, Tensor, Tensor> top_logits_distillation_stats_meta(const Tensor& logits, const Tensor& teacher, const Tensor& index,
+                                                                      double temperature, int64_t reduction) {
+  Tensor loss = top_logits_distillation_meta(logits, teacher, index, temperature, reduction);
+  return {loss, at::empty({logits.size(0), 2}, loss.options()), at::empty({on_device(logits) ? 2 : 1}, loss.options())};
+}
+Tensor top_logits_distillation_backward_meta(const Tensor& grad, const Tensor& logits, const Tensor& stats, const Tensor& count, const Tensor& teacher,
+                                             const Tensor& index, double temperature, int64_t reduction) {
+  check_distill_grads({logits, teacher, index, temperature, reduction}, grad, stats, count);
+  return at::empty(logits.sizes(), logits.options());
 }
 
 struct DistillNode : public torch::autograd::Node {
@@ -790,44 +859,58 @@ struct DistillNode : public torch::autograd::Node {
     if (!g[0].defined()) return out;
     const Tensor z = logits.unpack(), t = teacher.unpack(), i = index.unpack(), st = stats.unpack(), n = count.unpack();
     refuse_captured_backward("top_logits_distillation", z);
+    static const auto op = find_op<decltype(top_logits_distillation_backward)>("catch_b200::top_logits_distillation_backward");
     {
       Below below;
-      out[0] = distill_bwd({z, t, i, temperature, reduction}, g[0], st, n, std::exchange(ready, Tensor()));
+      // (an early gradient is there only if nothing but the kernels saw the forward)
+      if (ready.defined() && plain(z) && plain(g[0])) out[0] = distill_bwd({z, t, i, temperature, reduction}, g[0], st, n, std::exchange(ready, Tensor()));
+      else out[0] = op.call(g[0], z, st, n, t, i, temperature, reduction);
     }
     return once_differentiable("top_logits_distillation", std::move(out));
   }
 };
 
-Tensor top_logits_distillation(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction) {
-  return std::get<0>(distill_fwd({logits, teacher, index, temperature, reduction}, false));
+// Records the node of a loss.
+void record_distill(const Tensor& loss, const Tensor& logits, const Tensor& teacher, const Tensor& index, const Tensor& stats, const Tensor& count,
+                    Tensor ready, double temperature, int64_t reduction) {
+  auto node = make_node<DistillNode>();
+  node->set_next_edges(torch::autograd::collect_next_edges(logits));
+  node->logits = save(logits); node->teacher = save(teacher); node->index = save(index); node->stats = save(stats); node->count = save(count);
+  node->ready = std::move(ready);
+  node->temperature = temperature;
+  node->reduction = reduction;
+  torch::autograd::set_history(loss, node);
 }
-std::tuple<Tensor, Tensor, Tensor> top_logits_distillation_stats(const Tensor& logits, const Tensor& teacher, const Tensor& index,
-                                                                 double temperature, int64_t reduction) {
-  auto [loss, stats, count, ready] = distill_fwd({logits, teacher, index, temperature, reduction}, false);
+void refuse_teacher_grads(const Tensor& logits, const Tensor& teacher) {
+  refuse_tangents("top_logits_distillation", {&logits, &teacher});
+  TORCH_CHECK(!teacher.requires_grad(), "top_logits_distillation: the teacher's logits get no gradient; detach them");
+}
+std::tuple<Tensor, Tensor, Tensor> top_logits_distillation_stats_autograd(const Tensor& logits, const Tensor& teacher, const Tensor& index,
+                                                                          double temperature, int64_t reduction) {
+  refuse_teacher_grads(logits, teacher);
+  static const auto op = find_op<decltype(top_logits_distillation_stats)>("catch_b200::top_logits_distillation_stats");
+  Tensor loss, stats, count;
+  {
+    Below below;
+    std::tie(loss, stats, count) = op.call(logits, teacher, index, temperature, reduction);
+  }
+  if (wants_grad({&logits})) record_distill(loss, logits, teacher, index, stats, count, Tensor(), temperature, reduction);
   return {loss, stats, count};
-}
-Tensor top_logits_distillation_backward(const Tensor& grad, const Tensor& logits, const Tensor& stats, const Tensor& count, const Tensor& teacher,
-                                        const Tensor& index, double temperature, int64_t reduction) {
-  return distill_bwd({logits, teacher, index, temperature, reduction}, grad, stats, count, Tensor());
 }
 Tensor top_logits_distillation_autograd(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature,
                                         int64_t reduction) {
-  refuse_tangents("top_logits_distillation", {&logits, &teacher});
+  if (!plain(logits) || !plain(teacher) || !plain(index)) {  // an early gradient would be a constant to whatever else looks on
+    static const auto op = find_op<decltype(top_logits_distillation_stats)>("catch_b200::top_logits_distillation_stats");
+    return std::get<0>(op.call(logits, teacher, index, temperature, reduction));
+  }
+  refuse_teacher_grads(logits, teacher);
   const bool grad = wants_grad({&logits});
   Tensor loss, stats, count, ready;
   {
     Below below;
     std::tie(loss, stats, count, ready) = distill_fwd({logits, teacher, index, temperature, reduction}, grad);
   }
-  if (grad) {
-    auto node = make_node<DistillNode>();
-    node->set_next_edges(torch::autograd::collect_next_edges(logits));
-    node->logits = save(logits); node->teacher = save(teacher); node->index = save(index); node->stats = save(stats); node->count = save(count);
-    node->ready = ready;
-    node->temperature = temperature;
-    node->reduction = reduction;
-    torch::autograd::set_history(loss, node);
-  }
+  if (grad) record_distill(loss, logits, teacher, index, stats, count, ready, temperature, reduction);
   return loss;
 }
 
@@ -837,7 +920,8 @@ TORCH_LIBRARY_FRAGMENT(catch_b200, m) {
   m.def("qk_norm_rotary(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor cos, Tensor sin, Tensor? positions=None, "
         "float eps=1e-06, bool interleaved=False) -> (Tensor, Tensor)");
   m.def("qk_norm_rotary_backward(Tensor grad_q, Tensor grad_k, Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor cos, "
-        "Tensor sin, Tensor? positions, float eps, bool interleaved) -> (Tensor, Tensor, Tensor, Tensor)");
+        "Tensor sin, Tensor? positions, float eps, bool interleaved, bool need_q_weight=True, bool need_k_weight=True) -> "
+        "(Tensor, Tensor, Tensor, Tensor)");
   // (probabilities, statistics of the rows for the backward)
   m.def("relative_bias_softmax(Tensor scores, Tensor table, Tensor? mask=None, float scale=1.0, bool bidirectional=True, "
         "int max_distance=128, int query_offset=0) -> (Tensor, Tensor)");
@@ -863,7 +947,18 @@ TORCH_LIBRARY_IMPL(catch_b200, CompositeExplicitAutograd, m) {
   m.impl("top_logits_distillation", TORCH_FN(top_logits_distillation));
 }
 
+TORCH_LIBRARY_IMPL(catch_b200, Meta, m) {
+  m.impl("qk_norm_rotary", TORCH_FN(qk_norm_rotary_meta));
+  m.impl("qk_norm_rotary_backward", TORCH_FN(qk_norm_rotary_backward_meta));
+  m.impl("relative_bias_softmax", TORCH_FN(relative_bias_softmax_meta));
+  m.impl("relative_bias_softmax_backward", TORCH_FN(relative_bias_softmax_backward_meta));
+  m.impl("top_logits_distillation", TORCH_FN(top_logits_distillation_meta));
+  m.impl("top_logits_distillation_stats", TORCH_FN(top_logits_distillation_stats_meta));
+  m.impl("top_logits_distillation_backward", TORCH_FN(top_logits_distillation_backward_meta));
+}
+
 TORCH_LIBRARY_IMPL(catch_b200, Autograd, m) {
+  m.impl("top_logits_distillation_stats", TORCH_FN(top_logits_distillation_stats_autograd));
   m.impl("qk_norm_rotary", TORCH_FN(qk_norm_rotary_autograd));
   m.impl("relative_bias_softmax", TORCH_FN(relative_bias_softmax_autograd));
   m.impl("top_logits_distillation", TORCH_FN(top_logits_distillation_autograd));

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import transformer_cases as cases
+from test_transformer_ops_more import CALLS, _calls as calls
 from transformer_cases import check
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +44,33 @@ def test_logits_that_come_back_in_another_layout(dtype, factor, start, width):
                 loss = top_logits_distillation(leaf, t.to(DEV), idx.to(DEV), temperature=2.0)
                 (dz,) = torch.autograd.grad(loss, leaf, torch.tensor(factor).to(DEV))
             check(dz, *cases.distill_reference(z, t, idx, 2.0, "mean", factor)[1], "gradient")
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_function_transforms(name):
+    """As on the host; the same sums may be taken in another order where a slice lies elsewhere within 16 bytes."""
+    f, x = calls(DEV)[name]
+    g = torch.randn(f(x).shape).to(DEV)
+    total = lambda x: (f(x) * g).sum()  # noqa: E731
+    leaf = x.clone().requires_grad_()
+    (want,) = torch.autograd.grad(total(leaf), leaf)
+    near = lambda a, b: torch.allclose(a.cpu(), b.cpu(), rtol=2.0 ** -18, atol=2.0 ** -18)  # noqa: E731
+    assert near(torch.func.grad(total)(x), want)
+    value, pull = torch.func.vjp(f, x)
+    assert near(value, f(x)) and near(pull(g)[0], want)
+    many = torch.stack([x, 0.5 * x, -x])
+    assert near(torch.func.vmap(f)(many), torch.stack([f(v) for v in many]))
+    assert near(torch.func.vmap(torch.func.grad(total))(many), torch.stack([torch.func.grad(total)(v) for v in many]))
+
+
+def test_dispatch_modes_see_the_operators():
+    from test_transformer_ops_more import test_dispatch_modes_see_the_operators as on_host
+
+    on_host(DEV)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_fake_tensors_have_the_shapes(name):
+    from test_transformer_ops_more import test_fake_tensors_have_the_shapes as on_host
+
+    on_host(name, DEV)

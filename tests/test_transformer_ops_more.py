@@ -98,3 +98,129 @@ def test_forward_mode_is_refused_for_constants(what):
                 relative_bias_softmax(q, torch.zeros(4, 3), dual(torch.zeros(1, 1, 2, 8)))
             else:
                 top_logits_distillation(z, dual(torch.randn(3, 2)), torch.zeros(3, 2, dtype=torch.long))
+
+
+# --------------------------------------------------------------- what lies between autograd and the kernels sees the operators
+@pytest.mark.parametrize("dev", ["cpu", "blackwell"])
+@pytest.mark.parametrize("name", CALLS)
+def test_function_transforms(name, dev):
+    f, x = _calls(dev)[name]
+    g = torch.randn(f(x).shape).to(dev)
+    total = lambda x: (f(x) * g).sum()  # noqa: E731
+    leaf = x.clone().requires_grad_()
+    (want,) = torch.autograd.grad(total(leaf), leaf)
+    assert torch.equal(torch.func.grad(total)(x), want)
+    value, pull = torch.func.vjp(f, x)
+    assert torch.equal(value, f(x)) and torch.equal(pull(g)[0], want)
+    many = torch.stack([x, 0.5 * x, -x])
+    assert torch.equal(torch.func.vmap(f)(many), torch.stack([f(v) for v in many]))
+    each = torch.stack([torch.func.grad(total)(v) for v in many])
+    assert torch.allclose(torch.func.vmap(torch.func.grad(total))(many), each, rtol=2.0 ** -20, atol=2.0 ** -20)
+
+
+@pytest.mark.parametrize("dev", ["cpu", "blackwell"])
+def test_dispatch_modes_see_the_operators(dev):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    for name, (f, x) in _calls(dev).items():
+        want = f(x)
+        leaf = x.clone().requires_grad_()
+        with Seen() as seen:
+            y = f(leaf)
+            (d,) = torch.autograd.grad(y.sum(), leaf)
+        assert torch.equal(y, want) and d.shape == x.shape
+        op = {"rot": "qk_norm_rotary", "sof": "relative_bias_softmax", "dis": "top_logits_distillation"}[name[:3]]
+        ours = [n for n in seen.names if n.startswith("catch_b200::" + op)]
+        assert any(not n.endswith("_backward") for n in ours) and any(n.endswith("_backward") for n in ours), (name, seen.names)
+
+
+@pytest.mark.parametrize("dev", ["cpu", "blackwell"])
+@pytest.mark.parametrize("name", CALLS)
+def test_fake_tensors_have_the_shapes(name, dev):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.utils._pytree import tree_map
+
+    f, x = _calls(dev)[name]
+    leaf = x.clone().requires_grad_()
+    y = f(leaf)
+    (d,) = torch.autograd.grad(y.sum(), leaf)
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        fake = mode.from_tensor(x).requires_grad_()
+        fy = f(fake)
+        (fd,) = torch.autograd.grad(fy.sum(), fake)
+    for a, b in ((fy, y), (fd, d)):
+        assert a.shape == b.shape and a.dtype == b.dtype and a.device == b.device and a.stride() == b.stride()
+
+
+def test_meta_tensors_have_the_shapes_and_are_checked():
+    ops = torch.ops.catch_b200
+    m = dict(device="meta")
+    q, k, c, w = torch.randn(2, 5, 4, 8, **m), torch.randn(2, 5, 2, 8, **m), torch.randn(7, 3, **m), torch.randn(8, **m).bfloat16()
+    yq, yk = ops.qk_norm_rotary(q, k, w, None, c, c)
+    assert yq.shape == q.shape and yk.shape == k.shape
+    dq, dk, dw, none = ops.qk_norm_rotary_backward(yq, yk, q, k, w, None, c, c, None, 1e-6, False)
+    assert dq.shape == q.shape and dk.shape == k.shape and dw.shape == w.shape and dw.dtype == w.dtype and none is None
+    s, t = torch.randn(2, 3, 5, 6, **m).bfloat16(), torch.randn(8, 3, **m)
+    p, st = ops.relative_bias_softmax(s, t)
+    assert p.shape == s.shape and p.dtype == s.dtype and st.shape == (2, 3, 5, 2) and st.dtype == torch.float32
+    ds, dt = ops.relative_bias_softmax_backward(p, s, st, t, None, 1.0, True, 128, 0, True)
+    assert ds.shape == s.shape and dt.shape == t.shape
+    z, te, i = torch.randn(4, 9, **m).half(), torch.randn(4, 2, **m), torch.zeros(4, 2, dtype=torch.long, **m)
+    for reduction, shape in ((0, (4,)), (1, ()), (2, ())):
+        assert ops.top_logits_distillation(z, te, i, 1.0, reduction).shape == shape
+        loss, stats, count = ops.top_logits_distillation_stats(z, te, i, 1.0, reduction)
+        assert loss.shape == shape and loss.dtype == torch.float32 and stats.shape == (4, 2)
+        dz = ops.top_logits_distillation_backward(loss, z, stats, count, te, i, 1.0, reduction)
+        assert dz.shape == z.shape and dz.dtype == z.dtype
+    with pytest.raises(RuntimeError, match="differ in batch, length or head_dim"):
+        ops.qk_norm_rotary(q, k[:, :4], None, None, c, c)
+    with pytest.raises(RuntimeError, match="buckets, heads"):
+        ops.relative_bias_softmax(s, t[:, :2])
+    with pytest.raises(RuntimeError, match="shape of its logits"):
+        ops.top_logits_distillation(z, te, i[:, :1])
+
+
+def test_the_loss_with_its_statistics_is_differentiable():
+    z, te, idx = torch.randn(3, 7, requires_grad=True), torch.randn(3, 2), torch.tensor([[0, 3], [1, -1], [-1, -1]])
+    for reduction in (0, 1, 2):
+        plain = torch.ops.catch_b200.top_logits_distillation(z, te, idx, 2.0, reduction)
+        loss, stats, count = torch.ops.catch_b200.top_logits_distillation_stats(z, te, idx, 2.0, reduction)
+        assert not stats.requires_grad and not count.requires_grad
+        assert torch.equal(torch.autograd.grad(loss.sum(), z)[0], torch.autograd.grad(plain.sum(), z)[0])
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_traced_by_the_compiler(name):
+    f, x = _calls()[name]
+    g = torch.randn(f(x).shape)
+    total = lambda x: (f(x) * g).sum()  # noqa: E731
+    got = torch.compile(total, backend="aot_eager", fullgraph=True)
+    a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
+    total(a).backward()
+    got(b).backward()
+    assert torch.allclose(a.grad, b.grad, rtol=2.0 ** -20, atol=2.0 ** -20)
+
+
+def test_selective_checkpointing_keeps_the_results():
+    from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
+
+    def policy(ctx, op, *args, **kwargs):
+        return CheckpointPolicy.MUST_SAVE if "relative_bias_softmax" in op.name() else CheckpointPolicy.PREFER_RECOMPUTE
+
+    from catch_b200.fusion import relative_bias_softmax
+
+    torch.manual_seed(1)
+    s, t = torch.randn(1, 2, 3, 4, requires_grad=True), torch.randn(8, 2, requires_grad=True)
+    body = lambda s, t: relative_bias_softmax(s.sin(), t, max_distance=8).square().sum()  # noqa: E731
+    want = torch.autograd.grad(body(s, t), (s, t))
+    y = checkpoint(body, s, t, use_reentrant=False, context_fn=lambda: create_selective_checkpoint_contexts(policy))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (s, t)), want))

@@ -12,7 +12,6 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
 #include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
@@ -45,21 +44,6 @@ Tensor fresh(at::IntArrayRef sizes, const Tensor& like) { return empty_b200(size
 Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return empty_b200(sizes, type, like.device().index()); }
 Tensor fresh_strided(const Tensor& like) { return empty_strided_b200(like.sizes(), like.strides(), like.scalar_type(), like.device().index()); }
 bool on_device(const Tensor& t) { return !use_cpu_path() && is_b200(t); }
-
-// Results of a backward that is itself differentiated raise instead of counting as constants.
-variable_list once_differentiable(const char* op, variable_list grads) {
-  if (!at::GradMode::is_enabled()) return grads;
-  variable_list defined;
-  for (auto& g : grads)
-    if (g.defined()) defined.push_back(g.detach().set_requires_grad(true));
-  auto error = std::make_shared<torch::autograd::DelayedError>(
-      std::string(op) + ": the gradient of the gradient is not implemented", (int64_t)defined.size());
-  variable_list marked = (*error)(std::move(defined));
-  size_t n = 0;
-  for (auto& g : grads)
-    if (g.defined()) g = marked[n++];
-  return grads;
-}
 
 // ------------------------------------------------------------------------------------------ norm and rotation of q, k
 struct RotaryArgs {
@@ -276,18 +260,46 @@ const Tensor& or_none(const OptTensor& t) {
   static const Tensor none;
   return given(t) ? *t : none;
 }
+// Calls go on below autograd.
+using Below = at::AutoDispatchBelowADInplaceOrView;
 // An output without a tangent would count as one that does not depend on the inputs.
 void refuse_tangents(const char* op, std::initializer_list<const Tensor*> inputs) {
   for (const Tensor* t : inputs)
     TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), op, ": forward-mode derivatives are not implemented");
 }
+// The node of a gradient.  It leads to what the gradient was computed from, so that whoever differentiates it arrives here instead of
+// taking it for a constant.
+struct NoSecondDerivative : public torch::autograd::Node {
+  std::string op;
+  std::string name() const override { return "NoSecondDerivative"; }
+  variable_list apply(variable_list&&) override { TORCH_CHECK(false, op, ": the gradient of the gradient is not implemented"); }
+};
 template <typename N>
 std::shared_ptr<N> make_node() {
   return std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
 }
+// The autograd kernel of a _backward form: calls it below autograd and marks its results.
+template <typename F>
+auto first_derivative_only(const char* op, std::initializer_list<const Tensor*> inputs, F&& below) {
+  refuse_tangents(op, inputs);
+  auto grads = [&] {
+    Below guard;
+    return below();
+  }();
+  if (wants_grad(inputs)) {
+    auto node = make_node<NoSecondDerivative>();
+    node->op = op;
+    for (const Tensor* t : inputs)
+      if (t->defined()) node->add_next_edge(torch::autograd::impl::gradient_edge(*t));
+    auto mark = [&](const Tensor& g) {
+      if (g.defined()) torch::autograd::set_history(g, node);
+    };
+    if constexpr (std::is_same_v<std::decay_t<decltype(grads)>, Tensor>) mark(grads);
+    else std::apply([&](const auto&... g) { (mark(g), ...); }, grads);
+  }
+  return grads;
+}
 SavedVariable save(const Tensor& t) { return SavedVariable(t, /*is_output=*/false); }
-// Calls go on below autograd.
-using Below = at::AutoDispatchBelowADInplaceOrView;
 template <typename F>
 c10::TypedOperatorHandle<F> find_op(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
@@ -306,6 +318,15 @@ void refuse_captured_backward(const char* op, const Tensor& t) {
               "_backward instead");
 }
 
+std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_backward_autograd(const Tensor& dyq, const Tensor& dyk, const Tensor& q, const Tensor& k,
+                                                                            const OptTensor& qw, const OptTensor& kw, const Tensor& cos,
+                                                                            const Tensor& sin, const OptTensor& positions, double eps,
+                                                                            bool interleaved, bool need_qw, bool need_kw) {
+  static const auto op = find_op<decltype(qk_norm_rotary_backward)>("catch_b200::qk_norm_rotary_backward");
+  return first_derivative_only("qk_norm_rotary_backward", {&dyq, &dyk, &q, &k, &or_none(qw), &or_none(kw), &cos, &sin},
+                               [&] { return op.call(dyq, dyk, q, k, qw, kw, cos, sin, positions, eps, interleaved, need_qw, need_kw); });
+}
+
 struct RotaryNode : public torch::autograd::Node {
   SavedVariable q, k, qw, kw, cos, sin, positions;
   double eps = 0;
@@ -322,15 +343,12 @@ struct RotaryNode : public torch::autograd::Node {
     const Tensor uq = q.unpack(), uk = k.unpack();
     refuse_captured_backward("qk_norm_rotary", uq);
     static const auto op = find_op<decltype(qk_norm_rotary_backward)>("catch_b200::qk_norm_rotary_backward");
-    {
-      Below below;
-      Tensor gq = g[0].defined() ? g[0] : at::zeros_like(uq, at::MemoryFormat::Contiguous);
-      Tensor gk = g[1].defined() ? g[1] : at::zeros_like(uk, at::MemoryFormat::Contiguous);
-      std::tie(out[0], out[1], out[2], out[3]) =
-          op.call(gq, gk, uq, uk, saved_optional(qw.unpack()), saved_optional(kw.unpack()), cos.unpack(), sin.unpack(),
-                  saved_optional(positions.unpack()), eps, interleaved, task_should_compute_output(2), task_should_compute_output(3));
-    }
-    return once_differentiable("qk_norm_rotary", std::move(out));
+    const Tensor gq = g[0].defined() ? g[0] : at::zeros_like(uq, at::MemoryFormat::Contiguous);
+    const Tensor gk = g[1].defined() ? g[1] : at::zeros_like(uk, at::MemoryFormat::Contiguous);
+    std::tie(out[0], out[1], out[2], out[3]) =
+        op.call(gq, gk, uq, uk, saved_optional(qw.unpack()), saved_optional(kw.unpack()), cos.unpack(), sin.unpack(),
+                saved_optional(positions.unpack()), eps, interleaved, task_should_compute_output(2), task_should_compute_output(3));
+    return out;
   }
 };
 
@@ -598,6 +616,15 @@ std::tuple<Tensor, Tensor> relative_bias_softmax_backward(const Tensor& grad, co
   return {ds, dt};
 }
 
+std::tuple<Tensor, Tensor> relative_bias_softmax_backward_autograd(const Tensor& grad, const Tensor& scores, const Tensor& stats, const Tensor& table,
+                                                                   const OptTensor& mask, double scale, bool bidirectional, int64_t max_distance,
+                                                                   int64_t query_offset, bool need_table) {
+  static const auto op = find_op<decltype(relative_bias_softmax_backward)>("catch_b200::relative_bias_softmax_backward");
+  return first_derivative_only("relative_bias_softmax_backward", {&grad, &scores, &stats, &table, &or_none(mask)}, [&] {
+    return op.call(grad, scores, stats, table, mask, scale, bidirectional, max_distance, query_offset, need_table);
+  });
+}
+
 struct BiasNode : public torch::autograd::Node {
   SavedVariable scores, table, mask, stats;
   double scale = 1;
@@ -615,12 +642,9 @@ struct BiasNode : public torch::autograd::Node {
     const Tensor s = scores.unpack(), t = table.unpack(), m = mask.unpack(), st = stats.unpack();
     refuse_captured_backward("relative_bias_softmax", s);
     static const auto op = find_op<decltype(relative_bias_softmax_backward)>("catch_b200::relative_bias_softmax_backward");
-    {
-      Below below;
-      std::tie(out[0], out[1]) =
-          op.call(g[0], s, st, t, saved_optional(m), scale, bidirectional, max_distance, query_offset, task_should_compute_output(1));
-    }
-    return once_differentiable("relative_bias_softmax", std::move(out));
+    std::tie(out[0], out[1]) =
+        op.call(g[0], s, st, t, saved_optional(m), scale, bidirectional, max_distance, query_offset, task_should_compute_output(1));
+    return out;
   }
 };
 
@@ -842,6 +866,13 @@ Tensor top_logits_distillation_backward_meta(const Tensor& grad, const Tensor& l
   return at::empty(logits.sizes(), logits.options());
 }
 
+Tensor top_logits_distillation_backward_autograd(const Tensor& grad, const Tensor& logits, const Tensor& stats, const Tensor& count,
+                                                 const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction) {
+  static const auto op = find_op<decltype(top_logits_distillation_backward)>("catch_b200::top_logits_distillation_backward");
+  return first_derivative_only("top_logits_distillation_backward", {&grad, &logits, &stats, &count, &teacher},
+                               [&] { return op.call(grad, logits, stats, count, teacher, index, temperature, reduction); });
+}
+
 struct DistillNode : public torch::autograd::Node {
   SavedVariable logits, teacher, index, stats, count;
   Tensor ready;  // the gradient for a factor of 1, handed out once: a second pass over a retained graph writes one of its own
@@ -860,13 +891,15 @@ struct DistillNode : public torch::autograd::Node {
     const Tensor z = logits.unpack(), t = teacher.unpack(), i = index.unpack(), st = stats.unpack(), n = count.unpack();
     refuse_captured_backward("top_logits_distillation", z);
     static const auto op = find_op<decltype(top_logits_distillation_backward)>("catch_b200::top_logits_distillation_backward");
-    {
+    // The early gradient, if nobody but the kernels looks on; it is a constant to whoever differentiates once more.
+    if (ready.defined() && !at::GradMode::is_enabled() && plain(z) && plain(g[0])) {
+      refuse_tangents("top_logits_distillation", {&g[0]});
       Below below;
-      // (an early gradient is there only if nothing but the kernels saw the forward)
-      if (ready.defined() && plain(z) && plain(g[0])) out[0] = distill_bwd({z, t, i, temperature, reduction}, g[0], st, n, std::exchange(ready, Tensor()));
-      else out[0] = op.call(g[0], z, st, n, t, i, temperature, reduction);
+      out[0] = distill_bwd({z, t, i, temperature, reduction}, g[0], st, n, std::exchange(ready, Tensor()));
+    } else {
+      out[0] = op.call(g[0], z, st, n, t, i, temperature, reduction);
     }
-    return once_differentiable("top_logits_distillation", std::move(out));
+    return out;
   }
 };
 
@@ -958,6 +991,9 @@ TORCH_LIBRARY_IMPL(catch_b200, Meta, m) {
 }
 
 TORCH_LIBRARY_IMPL(catch_b200, Autograd, m) {
+  m.impl("qk_norm_rotary_backward", TORCH_FN(qk_norm_rotary_backward_autograd));
+  m.impl("relative_bias_softmax_backward", TORCH_FN(relative_bias_softmax_backward_autograd));
+  m.impl("top_logits_distillation_backward", TORCH_FN(top_logits_distillation_backward_autograd));
   m.impl("top_logits_distillation_stats", TORCH_FN(top_logits_distillation_stats_autograd));
   m.impl("qk_norm_rotary", TORCH_FN(qk_norm_rotary_autograd));
   m.impl("relative_bias_softmax", TORCH_FN(relative_bias_softmax_autograd));

@@ -74,3 +74,17 @@ def test_fake_tensors_have_the_shapes(name):
     from test_transformer_ops_more import test_fake_tensors_have_the_shapes as on_host
 
     on_host(name, DEV)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_second_derivatives_are_refused(name):
+    from test_transformer_ops_more import test_second_derivatives_are_refused_however_they_are_asked_for as on_host
+
+    on_host(name, DEV)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_forward_mode_is_refused(name):
+    from test_transformer_ops_more import test_forward_mode_is_refused as on_host
+
+    on_host(name, DEV)

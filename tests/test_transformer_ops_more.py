@@ -224,3 +224,59 @@ def test_selective_checkpointing_keeps_the_results():
     want = torch.autograd.grad(body(s, t), (s, t))
     y = checkpoint(body, s, t, use_reentrant=False, context_fn=lambda: create_selective_checkpoint_contexts(policy))
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (s, t)), want))
+
+
+# ------------------------------------------------------------------------------------------------ derivatives of derivatives
+@pytest.mark.parametrize("dev", ["cpu", "blackwell"])
+@pytest.mark.parametrize("name", CALLS)
+def test_second_derivatives_are_refused_however_they_are_asked_for(name, dev):
+    import torch.autograd.forward_ad as fwd
+
+    f, x = _calls(dev)[name]
+    g = torch.randn(f(x).shape).to(dev)
+    total = lambda x: (f(x) * g).sum()  # noqa: E731
+    refused = lambda: pytest.raises(RuntimeError, match="gradient of the gradient|forward-mode")  # noqa: E731
+    with refused():
+        torch.func.grad(lambda x: torch.func.grad(total)(x).square().sum())(x)
+    with refused():
+        torch.func.jvp(torch.func.grad(total), (x,), (torch.ones_like(x),))
+    with refused():
+        torch.func.hessian(total)(x)
+    with refused():
+        torch.func.jacrev(torch.func.grad(total))(x)
+    with refused():  # of the gradient with respect to the factor that it starts from
+        torch.func.jvp(lambda g: torch.func.vjp(f, x)[1](g)[0], (g,), (g,))
+    leaf = x.clone().requires_grad_()
+    (d,) = torch.autograd.grad(total(leaf), leaf, create_graph=True)
+    with refused():
+        torch.autograd.grad(d.sum(), leaf, allow_unused=True)
+    start = g.clone().requires_grad_()
+    (d,) = torch.autograd.grad(f(leaf), leaf, start, create_graph=True)
+    with refused():
+        torch.autograd.grad(d.sum(), start)
+    with fwd.dual_level(), refused():
+        torch.autograd.grad(f(leaf), leaf, fwd.make_dual(g, torch.ones_like(g)))
+    # the value beside the gradient can be differentiated once more
+    both = lambda x: sum(t.sum() for t in torch.func.vjp(f, x)[:1])  # noqa: E731
+    assert torch.allclose(torch.func.grad(both)(x), torch.autograd.grad(f(leaf).sum(), leaf)[0], rtol=2.0 ** -20, atol=2.0 ** -20)
+
+
+def test_results_of_the_backward_forms_refuse_derivatives():
+    ops = torch.ops.catch_b200
+    cos, sin = cases.tables(4, 4)
+    q, w = torch.randn(1, 3, 2, 8, requires_grad=True), torch.ones(8, requires_grad=True)
+    s, z = torch.randn(1, 2, 3, 4, requires_grad=True), torch.randn(3, 7, requires_grad=True)
+    t, te, idx = torch.randn(8, 2), torch.randn(3, 2), torch.zeros(3, 2, dtype=torch.long)
+    p, st = ops.relative_bias_softmax(s.detach(), t)
+    loss, stats, count = ops.top_logits_distillation_stats(z.detach(), te, idx, 1.0, 1)
+    calls = [lambda: ops.qk_norm_rotary_backward(q.detach(), q.detach(), q, q, w, None, cos, sin, None, 1e-6, False)[:3],
+             lambda: ops.relative_bias_softmax_backward(p, s, st, t, None, 1.0, True, 128, 0, True),
+             lambda: (ops.top_logits_distillation_backward(torch.ones(()), z, stats, count, te, idx, 1.0, 1),)]
+    for call in calls:
+        with torch.no_grad():
+            plain = call()
+        assert not any(r.requires_grad for r in plain)
+        for r, want in zip(call(), plain):
+            assert torch.equal(r.detach(), want)
+            with pytest.raises(RuntimeError, match="gradient of the gradient"):
+                r.sum().backward()

@@ -244,6 +244,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_backward(const Tensor&
   }
   Workspace ws((size_t)b200_qk_norm_rotary_workspace(&p), scope);
   B200_KERNEL_CHECK(b200_qk_norm_rotary_bwd(&p, ws.get(), scope.stream()));
+  if (p.bad_flag) report_bad_index("qk_norm_rotary_backward", q);
   return {dq, dk, dqw, dkw};
 }
 
@@ -835,6 +836,7 @@ Tensor distill_bwd(const DistillArgs& a, const Tensor& grad, const Tensor& stats
   p.grad_ld = each && N > 1 ? g.stride(0) : 0;
   p.skip_factor_one = keep;
   B200_KERNEL_CHECK(b200_distill_bwd(&p, scope.stream()));
+  if (p.bad_flag) report_bad_index("top_logits_distillation_backward", z);
   return out;
 }
 

@@ -88,3 +88,36 @@ def test_forward_mode_is_refused(name):
     from test_transformer_ops_more import test_forward_mode_is_refused as on_host
 
     on_host(name, DEV)
+
+
+def test_an_index_out_of_range_in_a_backward_raises_there_and_not_later():
+    """In synchronous mode; the flag on the device is shared by all operators that look things up."""
+    ops = torch.ops.catch_b200
+    cos, sin = torch.ones(4, 2).to(DEV), torch.zeros(4, 2).to(DEV)
+    q, far = torch.randn(1, 3, 2, 8).to(DEV), torch.tensor([[0, 1, 4]]).to(DEV)
+    z, te = torch.randn(2, 5).to(DEV), torch.randn(2, 2).to(DEV)
+    good, bad = torch.tensor([[0, 1], [2, -1]]).to(DEV), torch.tensor([[0, 1], [2, 5]]).to(DEV)
+    loss, stats, count = ops.top_logits_distillation_stats(z, te, good, 1.0, 1)
+    rotary = lambda pos: ops.qk_norm_rotary_backward(q, q, q, q, None, None, cos, sin, pos, 1e-6, False)  # noqa: E731
+    distill = lambda idx: ops.top_logits_distillation_backward(loss, z, stats, count, te, idx, 1.0, 1)  # noqa: E731
+    rows, first = torch.randn(5, 3).to(DEV), torch.tensor([0, 4]).to(DEV)
+    torch.b200.set_flag("async_disable", True)
+    try:
+        for call, name in ((lambda: rotary(far), "qk_norm_rotary_backward"), (lambda: distill(bad), "top_logits_distillation_backward")):
+            with pytest.raises(IndexError, match=name):
+                call()
+            assert torch.equal(rows.index_select(0, first).cpu(), rows.cpu()[[0, 4]])  # nothing is left behind
+        rotary(torch.tensor([[-1, 0, 3]]).to(DEV))
+        distill(good)
+    finally:
+        torch.b200.set_flag("async_disable", False)
+    # a forward that ran before the mode was switched on
+    leaf = z.clone().requires_grad_()
+    late = ops.top_logits_distillation(leaf, te, bad, 1.0, 0)
+    torch.b200.set_flag("async_disable", True)
+    try:
+        with pytest.raises(IndexError, match="top_logits_distillation_backward"):
+            torch.autograd.grad(late.sum(), leaf)
+        assert torch.equal(rows.index_select(0, first).cpu(), rows.cpu()[[0, 4]])
+    finally:
+        torch.b200.set_flag("async_disable", False)

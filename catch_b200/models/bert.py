@@ -98,11 +98,11 @@ class BertSelfAttention(nn.Module):
             q, k = qk_norm_rotary(q, k, self.query_norm, self.key_norm, self.rotary_cos, self.rotary_sin)
         return q, k, v
 
-    def _biased_probs(self, scores, mask):
-        """Softmax of unscaled [B, h, L, L] scores with the relative position bias."""
+    def _biased_probs(self, scores, mask, scale):
+        """Softmax of [B, h, L, L] scores, times ``scale``, with the relative position bias."""
         from catch_b200.fusion import relative_bias_softmax
 
-        return relative_bias_softmax(scores, self.relative_bias, mask, scale=1.0 / math.sqrt(self.d), max_distance=self.max_distance)
+        return relative_bias_softmax(scores, self.relative_bias, mask, scale=scale, max_distance=self.max_distance)
 
     def forward(self, x, mask=None):
         B, L, H = x.shape
@@ -113,7 +113,7 @@ class BertSelfAttention(nn.Module):
         q, k, v = (split(t) for t in self._project(x))
         scores = torch.bmm(q, k.transpose(1, 2))
         if self.position == "relative_bias":
-            probs = self._biased_probs(scores.view(B, self.h, L, L), mask).view(B * self.h, L, L)
+            probs = self._biased_probs(scores.view(B, self.h, L, L), mask, 1.0 / math.sqrt(self.d)).view(B * self.h, L, L)
         else:
             scores = scores * (1.0 / math.sqrt(self.d))
             if mask is not None:
@@ -158,10 +158,10 @@ class FusedBertSelfAttention(BertSelfAttention):
             return t.to(cd).permute(0, 2, 1, 3)
 
         q, k, v = (heads(t) for t in self._project(x))
+        scores = matmul_nd(q, k.transpose(-1, -2), 1.0 / math.sqrt(self.d))  # (scaled before they are rounded: the range of fp16)
         if self.position == "relative_bias":
-            probs = self._biased_probs(matmul_nd(q, k.transpose(-1, -2)), mask)  # scale, bias, mask and softmax in one kernel
+            probs = self._biased_probs(scores, mask, 1.0)  # bias, mask and softmax in one kernel
         else:
-            scores = matmul_nd(q, k.transpose(-1, -2), 1.0 / math.sqrt(self.d))
             if mask is not None:
                 scores = scores + mask.to(scores.dtype)
             with torch.autocast("blackwell", enabled=False):  # the softmax kernel computes in fp32 whatever the storage type

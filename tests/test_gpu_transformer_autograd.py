@@ -121,3 +121,29 @@ def test_an_index_out_of_range_in_a_backward_raises_there_and_not_later():
         assert torch.equal(rows.index_select(0, first).cpu(), rows.cpu()[[0, 4]])
     finally:
         torch.b200.set_flag("async_disable", False)
+
+
+def test_large_products_in_half_precision():
+    """Queries times keys of 64 x 40 x 40 = 102400, beyond fp16; scaled by 1 / sqrt(64) they are 12800, the same for every key, so that
+    the probabilities are those of the bias alone."""
+    from catch_b200.models.bert import BertConfig, BertSelfAttention, FusedBertSelfAttention
+
+    torch.manual_seed(2)
+    c = BertConfig(hidden_size=128, num_attention_heads=2, attention_probs_dropout_prob=0.0, position_embedding_type="relative_bias")
+    att = BertSelfAttention(c)
+    with torch.no_grad():
+        for p in (att.query, att.key):
+            p.weight.zero_()
+            p.bias.fill_(40.0)
+        att.relative_bias.copy_(torch.randn(32, 2))
+    x = torch.randn(2, 9, 128)
+    want = att(x).detach()
+    att.__class__ = FusedBertSelfAttention
+    att.to(DEV)
+    with torch.autocast(DEV, dtype=torch.float16):
+        y = att(x.to(DEV))
+    assert y.dtype == torch.float16
+    y.float().sum().backward()
+    # (values, probabilities and the product's result are rounded to 2^-11 each; means of nine values of size one)
+    assert float((y.detach().cpu().float() - want).abs().max()) <= 4 * 2.0 ** -11 * float(want.abs().max().clamp(min=1.0))
+    assert all(bool(torch.isfinite(p.grad.cpu()).all()) for p in att.parameters())

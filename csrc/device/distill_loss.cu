@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
         }
         counted = true;
       }
-      T* d = static_cast<T*>(p.dlogits) + row * p.ld;
+      T* d = static_cast<T*>(p.dlogits) + row * p.dlogits_ld;
       T* d_body = d + r.head;
       const float factor = any ? (FWD ? 1.f : p.grad[p.grad_per_row ? row * p.grad_ld : 0]) * count_inv * p.temperature : 0.f;
       const float scale = any ? factor / s : 0.f;

@@ -600,7 +600,8 @@ typedef struct B200Distill {
   float* stats;              // [N, 2]: maximum and sum of exponentials; forward: written, or null
   float* count;              // for a mean: the number of rows with entries (the forward writes it); else null
   unsigned* ticket;          // forward with a loss: one word of scratch
-  void* dlogits;             // [N][ld] of dtype, at the same 16-byte phase as logits; forward: written with factor 1, or null
+  void* dlogits;             // [N][dlogits_ld] of dtype, every row at the same 16-byte phase as the row of logits; forward: written
+  int64_t dlogits_ld;        // with factor 1, or null
   const float* grad;         // backward: the factor, one for each row (grad_ld apart) or one for all
   int64_t grad_ld;
   int grad_per_row;

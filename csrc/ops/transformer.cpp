@@ -733,17 +733,21 @@ Tensor row_layout(const Tensor& t) {
   if ((t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1))) return t;
   return t.contiguous();
 }
-// An uninitialised tensor with the row distance of `t` whose rows begin at the same place within 16 bytes.
+// An uninitialised tensor whose rows begin at the same place within 16 bytes as those of `t`, which lie `ld` apart: as close
+// together as that allows (a token's logits of every sequence may lie a whole sequence apart).
 Tensor empty_in_phase(const Tensor& t, int64_t ld) {
-  const int64_t phase = (int64_t)(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) / (int64_t)t.element_size();
-  const int64_t rows = t.size(0), need = rows > 0 ? (rows - 1) * ld + t.size(1) : 0;
-  if (phase == 0 && ld == t.size(1)) return fresh(t.sizes(), t);
-  return fresh({need + phase}, t).as_strided(t.sizes(), {ld, 1}, phase);
+  const int64_t es = (int64_t)t.element_size(), vec = 16 / es, phase = (int64_t)(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) / es;
+  const int64_t rows = t.size(0), V = t.size(1), apart = V + (ld - V) % vec;
+  if (phase == 0 && apart == V) return fresh(t.sizes(), t);
+  return fresh({(rows > 0 ? (rows - 1) * apart + V : 0) + phase}, t).as_strided(t.sizes(), {apart, 1}, phase);
 }
+// The distance of the rows of [N, V] logits or of their gradient.
+int64_t row_distance(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
-// Whether `out` has the type, the rows' distance and the place within 16 bytes of `t`.
-bool same_rows(const Tensor& out, const Tensor& t, int64_t ld) {
-  return out.sizes() == t.sizes() && out.scalar_type() == t.scalar_type() && (out.size(0) <= 1 || out.stride(0) == ld) && (out.size(1) <= 1 || out.stride(1) == 1) &&
+// Whether `out` has the type of `t` and every row at the same place within 16 bytes.
+bool in_phase(const Tensor& out, const Tensor& t) {
+  return out.sizes() == t.sizes() && out.scalar_type() == t.scalar_type() &&
+         (row_distance(out) - row_distance(t)) * (int64_t)t.element_size() % 16 == 0 &&
          (reinterpret_cast<uintptr_t>(out.data_ptr()) - reinterpret_cast<uintptr_t>(t.data_ptr())) % 16 == 0;
 }
 
@@ -751,7 +755,7 @@ B200Distill distill_params(const DistillArgs& a, const Tensor& z, const Tensor& 
   B200Distill p{};
   p.logits = z.data_ptr(); p.teacher = teacher.data_ptr(); p.index = index.data_ptr();
   p.N = z.size(0); p.V = z.size(1); p.K = (int)teacher.size(1);
-  p.ld = z.size(0) > 1 ? z.stride(0) : z.size(1);
+  p.ld = row_distance(z);
   p.teacher_ld = teacher.size(1); p.index_ld = index.size(1);
   p.dtype = to_b200_dtype(z.scalar_type());
   p.teacher_dtype = to_b200_dtype(teacher.scalar_type());
@@ -795,6 +799,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> distill_fwd(const DistillArgs& a, boo
   if (need_grad && !each && z.scalar_type() != at::kHalf) {
     grad = empty_in_phase(z, p.ld);
     p.dlogits = grad.data_ptr();
+    p.dlogits_ld = row_distance(grad);
   }
   B200_KERNEL_CHECK(b200_distill_fwd(&p, scope.stream()));
   if (p.bad_flag) report_bad_index("top_logits_distillation", z);
@@ -825,12 +830,13 @@ Tensor distill_bwd(const DistillArgs& a, const Tensor& grad, const Tensor& stats
   Tensor z = row_layout(a.logits), teacher = a.teacher.contiguous(), index = a.index.contiguous(), g = grad.to(at::kFloat);
   B200Distill p = distill_params(a, z, teacher, index);
   // What backward() is given may lie elsewhere than what the forward saw (hooks on saved tensors, a recomputed forward): the kernel
-  // takes the row distance and the place within 16 bytes of both from the logits.
-  const bool keep = ready.defined() && same_rows(ready, z, p.ld);
+  // takes the rows' place within 16 bytes from the logits.
+  const bool keep = ready.defined() && in_phase(ready, z);
   Tensor out = keep ? ready : empty_in_phase(z, p.ld);
   p.stats = stats.data_ptr<float>();
   p.count = mean ? count.data_ptr<float>() : nullptr;
   p.dlogits = out.data_ptr();
+  p.dlogits_ld = row_distance(out);
   p.grad = g.data_ptr<float>();
   p.grad_per_row = each;
   p.grad_ld = each && N > 1 ? g.stride(0) : 0;

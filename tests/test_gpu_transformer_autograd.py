@@ -147,3 +147,29 @@ def test_large_products_in_half_precision():
     # (values, probabilities and the product's result are rounded to 2^-11 each; means of nine values of size one)
     assert float((y.detach().cpu().float() - want).abs().max()) <= 4 * 2.0 ** -11 * float(want.abs().max().clamp(min=1.0))
     assert all(bool(torch.isfinite(p.grad.cpu()).all()) for p in att.parameters())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V, width, step", [(4096, 4096, 64), (1001, 1001, 37), (999, 1005, 5), (7, 1000, 1)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_the_gradient_takes_the_memory_of_the_logits(dtype, V, width, step, reduction):
+    """Whatever the distance of the logits' rows, such as that of each sequence's last token."""
+    from catch_b200.fusion import top_logits_distillation
+
+    N = 9
+    torch.manual_seed(V)
+    whole = torch.randn(N, step, width).to(dtype).to(DEV)
+    z = whole[:, step // 2, width - V:].detach().requires_grad_()
+    assert z.stride(0) == step * width
+    t, idx = cases.teacher_of(N, V, 5, 3)
+    t, idx = t.to(DEV), idx.to(DEV)
+    g = torch.rand(N).to(DEV) if reduction == "none" else torch.ones(()).to(DEV)
+    torch.b200.synchronize()
+    before = torch.b200.memory_allocated()
+    loss = top_logits_distillation(z, t, idx, temperature=2.0, reduction=reduction)
+    gradient = N * (V + 8) * z.element_size() + 16
+    assert torch.b200.memory_allocated() - before <= gradient + 8 * 512  # (the allocator's blocks are multiples of 512 bytes)
+    for factor in (1, 2):
+        (dz,) = torch.autograd.grad(loss, z, factor * g, retain_graph=True)
+        assert dz.untyped_storage().nbytes() <= gradient
+        check(dz, *cases.distill_reference(z, t, idx, 2.0, reduction, (factor * g).cpu())[1], "gradient")

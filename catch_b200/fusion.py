@@ -433,17 +433,22 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
 def top_logits_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor, *, temperature: float = 1.0,
-                            reduction: str = "mean") -> torch.Tensor:
+                            reduction: str = "mean", early_gradient: bool = True) -> torch.Tensor:
     """Distillation loss against a teacher of which the largest logits of every row are kept.
 
     ``logits`` ``[rows, vocabulary]``; ``teacher_logits`` / ``teacher_index`` ``[rows, kept]`` are the teacher's values and their places in
     the vocabulary (``torch.topk`` of its logits).  A row's loss is ``temperature ** 2 * sum(p * (log p - log q))`` with ``p`` the softmax
     of the kept logits and ``q`` the student's softmax over the whole vocabulary, both at ``temperature``.  An entry whose index is
     negative is absent, and a row without entries counts nothing: not in the loss, the gradient or the mean.  ``reduction``:
-    ``"mean"`` over the rows that count, ``"sum"`` or ``"none"``; the loss is fp32.  Differentiable in ``logits``."""
+    ``"mean"`` over the rows that count, ``"sum"`` or ``"none"``; the loss is fp32.  Differentiable in ``logits``.
+
+    ``early_gradient``: the forward of a mean or a sum (in bf16 and fp32) writes the gradient for ``loss.backward()``'s factor of 1 while
+    it has the row at hand, which saves a pass and holds a tensor of the logits' size until the backward.  Switch it off for a
+    loss that is weighted, divided (gradient accumulation), scaled or only logged: another factor writes the gradient anew."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"top_logits_distillation: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
-    return torch.ops.catch_b200.top_logits_distillation.default(logits, teacher_logits, teacher_index, temperature, _REDUCTIONS[reduction])
+    return torch.ops.catch_b200.top_logits_distillation.default(logits, teacher_logits, teacher_index, temperature, _REDUCTIONS[reduction],
+                                                                early_gradient)
 
 
 def _feeds_only(node: fx.Node, consumer: fx.Node) -> bool:

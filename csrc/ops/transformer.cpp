@@ -846,7 +846,8 @@ Tensor distill_bwd(const DistillArgs& a, const Tensor& grad, const Tensor& stats
   return out;
 }
 
-Tensor top_logits_distillation(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction) {
+Tensor top_logits_distillation(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction,
+                               bool /*early_gradient*/) {
   return std::get<0>(distill_fwd({logits, teacher, index, temperature, reduction}, false));
 }
 std::tuple<Tensor, Tensor, Tensor> top_logits_distillation_stats(const Tensor& logits, const Tensor& teacher, const Tensor& index,
@@ -858,14 +859,15 @@ Tensor top_logits_distillation_backward(const Tensor& grad, const Tensor& logits
                                         const Tensor& index, double temperature, int64_t reduction) {
   return distill_bwd({logits, teacher, index, temperature, reduction}, grad, stats, count, Tensor());
 }
-Tensor top_logits_distillation_meta(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction) {
+Tensor top_logits_distillation_meta(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction,
+                                    bool early_gradient) {
   check_distill({logits, teacher, index, temperature, reduction});
   auto opt = logits.options().dtype(at::kFloat);
   return reduction == at::Reduction::None ? at::empty({logits.size(0)}, opt) : at::empty({}, opt);
 }
 std::tuple<Tensor, Tensor, Tensor> top_logits_distillation_stats_meta(const Tensor& logits, const Tensor& teacher, const Tensor& index,
                                                                       double temperature, int64_t reduction) {
-  Tensor loss = top_logits_distillation_meta(logits, teacher, index, temperature, reduction);
+  Tensor loss = top_logits_distillation_meta(logits, teacher, index, temperature, reduction, false);
   return {loss, at::empty({logits.size(0), 2}, loss.options()), at::empty({on_device(logits) ? 2 : 1}, loss.options())};
 }
 Tensor top_logits_distillation_backward_meta(const Tensor& grad, const Tensor& logits, const Tensor& stats, const Tensor& count, const Tensor& teacher,
@@ -939,7 +941,7 @@ std::tuple<Tensor, Tensor, Tensor> top_logits_distillation_stats_autograd(const 
   return {loss, stats, count};
 }
 Tensor top_logits_distillation_autograd(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature,
-                                        int64_t reduction) {
+                                        int64_t reduction, bool early_gradient) {
   if (!plain(logits) || !plain(teacher) || !plain(index)) {  // an early gradient would be a constant to whatever else looks on
     static const auto op = find_op<decltype(top_logits_distillation_stats)>("catch_b200::top_logits_distillation_stats");
     return std::get<0>(op.call(logits, teacher, index, temperature, reduction));
@@ -949,7 +951,7 @@ Tensor top_logits_distillation_autograd(const Tensor& logits, const Tensor& teac
   Tensor loss, stats, count, ready;
   {
     Below below;
-    std::tie(loss, stats, count, ready) = distill_fwd({logits, teacher, index, temperature, reduction}, grad);
+    std::tie(loss, stats, count, ready) = distill_fwd({logits, teacher, index, temperature, reduction}, grad && early_gradient);
   }
   if (grad) record_distill(loss, logits, teacher, index, stats, count, ready, temperature, reduction);
   return loss;
@@ -968,9 +970,10 @@ TORCH_LIBRARY_FRAGMENT(catch_b200, m) {
         "int max_distance=128, int query_offset=0) -> (Tensor, Tensor)");
   m.def("relative_bias_softmax_backward(Tensor grad, Tensor scores, Tensor stats, Tensor table, Tensor? mask, float scale, "
         "bool bidirectional, int max_distance, int query_offset, bool need_table) -> (Tensor, Tensor)");
-  // reduction: 0 a loss for each row, 1 their mean over the rows with entries, 2 their sum
-  m.def("top_logits_distillation(Tensor logits, Tensor teacher_logits, Tensor teacher_index, float temperature=1.0, int reduction=1) "
-        "-> Tensor");
+  // reduction: 0 a loss for each row, 1 their mean over the rows with entries, 2 their sum; early_gradient: the forward writes the
+  // gradient for a factor of 1, where one is wanted
+  m.def("top_logits_distillation(Tensor logits, Tensor teacher_logits, Tensor teacher_index, float temperature=1.0, int reduction=1, "
+        "bool early_gradient=True) -> Tensor");
   // the loss with what its backward needs (statistics of the rows, number of rows that count), and that backward
   m.def("top_logits_distillation_stats(Tensor logits, Tensor teacher_logits, Tensor teacher_index, float temperature, int reduction) "
         "-> (Tensor, Tensor, Tensor)");

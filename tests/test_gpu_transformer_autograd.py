@@ -173,3 +173,25 @@ def test_the_gradient_takes_the_memory_of_the_logits(dtype, V, width, step, redu
         (dz,) = torch.autograd.grad(loss, z, factor * g, retain_graph=True)
         assert dz.untyped_storage().nbytes() <= gradient
         check(dz, *cases.distill_reference(z, t, idx, 2.0, reduction, (factor * g).cpu())[1], "gradient")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_without_the_early_gradient_the_forward_holds_none(dtype, reduction):
+    from catch_b200.fusion import top_logits_distillation
+
+    N, V = 64, 40000
+    z = torch.randn(N, V).to(dtype)
+    t, idx = cases.teacher_of(N, V, 5, 3)
+    leaf = z.to(DEV).requires_grad_()
+    args = (leaf, t.to(DEV), idx.to(DEV))
+    for early in (True, False):
+        torch.b200.synchronize()
+        before = torch.b200.memory_allocated()
+        loss = top_logits_distillation(*args, temperature=2.0, reduction=reduction, early_gradient=early)
+        assert (torch.b200.memory_allocated() - before >= z.numel() * z.element_size()) == early
+        for factor in (1.0, 0.3):
+            (dz,) = torch.autograd.grad(loss, leaf, torch.tensor(factor).to(DEV), retain_graph=True)
+            check(dz, *cases.distill_reference(z, t, idx, 2.0, reduction, factor)[1], "gradient")
+            del dz
+        del loss

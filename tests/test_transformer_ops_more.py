@@ -280,3 +280,16 @@ def test_results_of_the_backward_forms_refuse_derivatives():
             assert torch.equal(r.detach(), want)
             with pytest.raises(RuntimeError, match="gradient of the gradient"):
                 r.sum().backward()
+
+
+@pytest.mark.parametrize("dev", ["cpu", "blackwell"])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_the_early_gradient_can_be_left_out(dev, reduction):
+    from catch_b200.fusion import top_logits_distillation
+
+    z, te, idx = torch.randn(3, 7).to(dev).requires_grad_(), torch.randn(3, 2).to(dev), torch.tensor([[0, 3], [1, -1], [-1, -1]]).to(dev)
+    with_it, without = (top_logits_distillation(z, te, idx, temperature=2.0, reduction=reduction, early_gradient=e) for e in (True, False))
+    assert torch.equal(with_it, without)
+    for factor in (1.0, 0.3):
+        a, b = (torch.autograd.grad(factor * y.sum(), z, retain_graph=True)[0] for y in (with_it, without))
+        assert torch.equal(a, b)

@@ -44,7 +44,7 @@ class BertEmbeddings(nn.Module):
     def __init__(self, c: BertConfig):
         super().__init__()
         self.word_embeddings = nn.Embedding(c.vocab_size, c.hidden_size)
-        self.absolute = c.position_embedding_type == "absolute"
+        self.absolute = getattr(c, "position_embedding_type", "absolute") == "absolute"
         if self.absolute:
             self.position_embeddings = nn.Embedding(c.max_position_embeddings, c.hidden_size)
         self.token_type_embeddings = nn.Embedding(c.type_vocab_size, c.hidden_size)
@@ -74,7 +74,7 @@ class BertSelfAttention(nn.Module):
         self.key = nn.Linear(c.hidden_size, c.hidden_size)
         self.value = nn.Linear(c.hidden_size, c.hidden_size)
         self.dropout = nn.Dropout(c.attention_probs_dropout_prob)
-        self.position = c.position_embedding_type
+        self.position = getattr(c, "position_embedding_type", "absolute")  # (configurations from before there was a choice)
         if self.position == "relative_bias":
             self.max_distance = c.relative_attention_max_distance
             self.relative_bias = nn.Parameter(torch.zeros(c.relative_attention_num_buckets, self.h))

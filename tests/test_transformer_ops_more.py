@@ -293,3 +293,19 @@ def test_the_early_gradient_can_be_left_out(dev, reduction):
     for factor in (1.0, 0.3):
         a, b = (torch.autograd.grad(factor * y.sum(), z, retain_graph=True)[0] for y in (with_it, without))
         assert torch.equal(a, b)
+
+
+def test_an_encoder_takes_configurations_from_before_there_were_position_types():
+    from types import SimpleNamespace
+
+    from catch_b200.models.bert import BertConfig, BertForSequenceClassification
+
+    new = ("position_embedding_type", "relative_attention_num_buckets", "relative_attention_max_distance", "rotary_base")
+    c = BertConfig(vocab_size=50, hidden_size=16, num_hidden_layers=1, num_attention_heads=2, intermediate_size=32, max_position_embeddings=10)
+    old = SimpleNamespace(**{k: v for k, v in vars(c).items() if k not in new})
+    torch.manual_seed(0)
+    a = BertForSequenceClassification(c).eval()
+    b = BertForSequenceClassification(old).eval()
+    b.load_state_dict(a.state_dict())
+    ids = torch.randint(0, 50, (2, 7))
+    assert torch.equal(a(ids), b(ids))

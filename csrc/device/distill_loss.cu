@@ -161,6 +161,18 @@ struct Stream {
   }
 };
 
+// Rows are counted by up to 32 blocks, each of about 8192 entries.
+constexpr int kCountThreads = 1024;
+__host__ __device__ __forceinline__ int count_blocks(const B200Distill& p) {
+  const long long blocks = p.N * p.K / 8192 + 1;
+  return blocks < B200_DISTILL_SCRATCH - 1 ? (int)blocks : B200_DISTILL_SCRATCH - 1;
+}
+// Their sum; called by whole warps.
+__device__ __forceinline__ float rows_counted(const B200Distill& p) {
+  const int lane = threadIdx.x & 31;
+  return (float)__reduce_add_sync(0xffffffffu, lane < count_blocks(p) ? __ldcg(p.scratch + 1 + lane) : 0u);
+}
+
 template <typename T, int VEC, bool FWD, bool GRAD>
 __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_constant__ B200Distill p) {
   __shared__ Shared sh;
@@ -292,7 +304,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
       if (FWD && !counted) {  // the number of rows comes from the kernel in front, which may still run
         if (p.count) {
           cudaGridDependencySynchronize();
-          count_inv = 1.f / fmaxf(*static_cast<volatile const float*>(p.count), 1.f);
+          count_inv = 1.f / fmaxf(rows_counted(p), 1.f);
         }
         counted = true;
       }
@@ -348,11 +360,11 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
   }
   if (!FWD || !p.loss) return;
   // The block that ends last adds up the rows' losses, in an order that does not depend on which one it is.
-  cudaGridDependencySynchronize();  // the ticket was set by the kernel in front
+  cudaGridDependencySynchronize();  // ticket and numbers were set by the kernel in front
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
-    sh.last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
+    sh.last = atomicAdd(p.scratch, 1u) == gridDim.x - 1;
     __threadfence();
   }
   __syncthreads();
@@ -362,39 +374,66 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const __grid_co
   sum = group_sum(sum, 32);
   if (lane == 0) sh.loss[warp] = sum;
   __syncthreads();
+  const float count = p.count ? rows_counted(p) : 1.f;
   if (threadIdx.x == 0) {
     sum = 0.f;
     for (int w = 0; w < blockDim.x / 32; ++w) sum += sh.loss[w];
-    *p.loss = p.count ? sum / fmaxf(__ldcg(p.count), 1.f) : sum;
+    *p.loss = sum / fmaxf(count, 1.f);
+    if (p.count) *p.count = count;
   }
 }
 
-// The number of rows with at least one entry (for a mean), and the ticket of the blocks that follow.  One block: the kernel behind it
-// starts at once and needs the number only when its first gradients are written.
-__global__ void __launch_bounds__(1024) distill_count_kernel(const __grid_constant__ B200Distill p) {
+// The number of rows with at least one entry (for a mean), in a part for each block, and the ticket of the blocks that follow.  The kernel
+// behind starts at once and needs the number only when its first gradients are written.  A lane looks at the first entry of a row of its
+// own, which decides most rows; those that it leaves open are gone through by groups of lanes, four entries to a lane.  (A mean and its
+// gradient, bf16, 85 % of the rows without entries: 16384 x 4000, 128 kept, 1060 us with a thread for each row in one block, 153 us so;
+// 4096 x 30522, 64 kept: 228 and 122 us.)
+__global__ void __launch_bounds__(kCountThreads) distill_count_kernel(const __grid_constant__ B200Distill p) {
   cudaTriggerProgrammaticLaunchCompletion();
-  __shared__ int red[32];
-  if (threadIdx.x == 0) *p.ticket = 0;
+  __shared__ int red[kCountThreads / 32];
+  if (threadIdx.x == 0 && blockIdx.x == 0) p.scratch[0] = 0;
   if (!p.count) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int G = 1;
+  while (G < 32 && 4 * G < p.K - 1) G *= 2;
+  const long long warps = (long long)gridDim.x * (kCountThreads / 32), share = (p.N + warps - 1) / warps;
+  const int rows = share < 32 ? (int)share : 32;  // of a warp at a time
   int n = 0;
-#pragma unroll 4
-  for (long long row = threadIdx.x; row < p.N; row += blockDim.x) {
-    bool there = false;
-    for (int k = 0; !there && k < p.K; ++k) there = present(p, row, k);
-    n += there;
+  for (long long base = (blockIdx.x * (kCountThreads / 32) + warp) * (long long)rows; base < p.N; base += warps * rows) {
+    const bool mine = lane < rows && base + lane < p.N;
+    const bool first = mine && p.K > 0 && present(p, base + lane, 0);
+    n += first;
+    for (unsigned open = __ballot_sync(0xffffffffu, mine && !first); open;) {
+      const unsigned pick = __fns(open, 0, lane / G + 1);  // this group's row; none left: beyond 31
+      bool there = false;
+      if (pick < 32) {
+        const long long row = base + pick;
+        for (int k = 1 + lane % G; k < p.K; k += 4 * G) {
+          long long i[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) i[u] = k + u * G < p.K ? index_at(p, row, k + u * G) : -1;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            there |= i[u] >= 0 && i[u] < p.V && teacher_at(p.teacher, row * p.teacher_ld + k + u * G, p.teacher_dtype) != kNegInf;
+        }
+      }
+      const unsigned hits = __ballot_sync(0xffffffffu, there) >> (lane / G * G) & (0xffffffffu >> (32 - G));
+      n += lane % G == 0 && hits != 0;
+      for (int q = 0; q < 32 / G; ++q) open &= open - 1;
+    }
   }
   n = __reduce_add_sync(0xffffffffu, n);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = n;
+  if (lane == 0) red[warp] = n;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    n = __reduce_add_sync(0xffffffffu, red[threadIdx.x]);
-    if (threadIdx.x == 0) *p.count = (float)n;
+  if (warp == 0) {
+    n = __reduce_add_sync(0xffffffffu, red[lane]);
+    if (lane == 0) p.scratch[1 + blockIdx.x] = (unsigned)n;
   }
 }
 
 bool valid(const B200Distill* p) {
   return p->N >= 0 && p->V >= 1 && p->V < (1LL << 31) - 8192 && p->K >= 0 && p->K <= B200_DISTILL_MAX_K && p->temperature > 0.f &&
-         (p->index_dtype == B200_I64 || p->index_dtype == B200_I32) && (!p->loss || p->ticket);
+         (p->index_dtype == B200_I64 || p->index_dtype == B200_I32) && (!p->loss || p->scratch);
 }
 
 // Threads for a row: 30 vectors for each, and at least half as many as there are kept entries.  Small blocks because a row's
@@ -441,7 +480,7 @@ extern "C" int b200_distill_fwd(const B200Distill* p, void* stream) {
   cudaStream_t s = (cudaStream_t)stream;
   if (p->N == 0) return p->loss ? (int)cudaMemsetAsync(p->loss, 0, sizeof(float), s) : 0;
   if (p->loss) {
-    distill_count_kernel<<<1, 1024, 0, s>>>(*p);
+    distill_count_kernel<<<p->count ? count_blocks(*p) : 1, kCountThreads, 0, s>>>(*p);
     const int rc = (int)cudaGetLastError();
     if (rc) return rc;
   }

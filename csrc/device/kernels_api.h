@@ -586,6 +586,7 @@ B200_API int b200_bias_softmax_bwd(const B200BiasSoftmax* p, void* workspace, vo
 
 // Distillation loss against a teacher's top K logits (distill_loss.cu).
 #define B200_DISTILL_MAX_K 1024
+#define B200_DISTILL_SCRATCH 33
 typedef struct B200Distill {
   const void* logits;        // [N][ld], V columns used; f32 / bf16 / f16
   const void* teacher;       // [N][teacher_ld], K columns; f32 / bf16 / f16
@@ -599,7 +600,7 @@ typedef struct B200Distill {
   float* loss;               // sum (or mean) of the rows' losses, or null
   float* stats;              // [N, 2]: maximum and sum of exponentials; forward: written, or null
   float* count;              // for a mean: the number of rows with entries (the forward writes it); else null
-  unsigned* ticket;          // forward with a loss: one word of scratch
+  unsigned* scratch;         // forward with a loss: B200_DISTILL_SCRATCH words
   void* dlogits;             // [N][dlogits_ld] of dtype, every row at the same 16-byte phase as the row of logits; forward: written
   int64_t dlogits_ld;        // with factor 1, or null
   const float* grad;         // backward: the factor, one for each row (grad_ld apart) or one for all

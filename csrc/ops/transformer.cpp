@@ -786,14 +786,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> distill_fwd(const DistillArgs& a, boo
   }
   OpScope scope("top_logits_distillation", a.logits);
   Tensor z = row_layout(a.logits), teacher = a.teacher.contiguous(), index = a.index.contiguous();
-  Tensor rows = fresh({N}, at::kFloat, z), stats = fresh({N, 2}, at::kFloat, z), count = fresh({2}, at::kFloat, z);  // (count, scratch)
+  Tensor rows = fresh({N}, at::kFloat, z), stats = fresh({N, 2}, at::kFloat, z), count = fresh({1 + B200_DISTILL_SCRATCH}, at::kFloat, z);  // (count, scratch)
   Tensor loss = each ? rows : fresh({}, at::kFloat, z), grad;
   B200Distill p = distill_params(a, z, teacher, index);
   p.row_loss = rows.data_ptr<float>();
   p.stats = stats.data_ptr<float>();
   p.loss = each ? nullptr : loss.data_ptr<float>();
   p.count = mean ? count.data_ptr<float>() : nullptr;
-  p.ticket = reinterpret_cast<unsigned*>(count.data_ptr<float>() + 1);
+  p.scratch = reinterpret_cast<unsigned*>(count.data_ptr<float>() + 1);
   // The gradient for a factor of 1, while the row is in the caches.  Not in half precision: its training scales the loss, so that the
   // factor is another one, and a gradient rounded before the scaling would lose what the scaling is there to keep.
   if (need_grad && !each && z.scalar_type() != at::kHalf) {
@@ -868,7 +868,7 @@ Tensor top_logits_distillation_meta(const Tensor& logits, const Tensor& teacher,
 std::tuple<Tensor, Tensor, Tensor> top_logits_distillation_stats_meta(const Tensor& logits, const Tensor& teacher, const Tensor& index,
                                                                       double temperature, int64_t reduction) {
   Tensor loss = top_logits_distillation_meta(logits, teacher, index, temperature, reduction, false);
-  return {loss, at::empty({logits.size(0), 2}, loss.options()), at::empty({on_device(logits) ? 2 : 1}, loss.options())};
+  return {loss, at::empty({logits.size(0), 2}, loss.options()), at::empty({on_device(logits) ? 1 + B200_DISTILL_SCRATCH : 1}, loss.options())};
 }
 Tensor top_logits_distillation_backward_meta(const Tensor& grad, const Tensor& logits, const Tensor& stats, const Tensor& count, const Tensor& teacher,
                                              const Tensor& index, double temperature, int64_t reduction) {

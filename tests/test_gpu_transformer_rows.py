@@ -178,3 +178,24 @@ def test_mask_bytes_beyond_two_to_the_31(mask_dtype):
     ds = ds.cpu().flatten()
     assert int((ds != 0).sum()) == last + some
     assert abs(float(ds[-1]) - q * (1 - q)) <= q * 2.0 ** -8 and abs(float(ds[-2]) + q * q) <= q * q * 2.0 ** -7
+
+
+@pytest.mark.parametrize("N, K", [(1, 1), (33, 1), (40, 2), (1000, 5), (700, 6), (300, 33), (5000, 64), (3000, 130), (16411, 17), (9, 1024), (70000, 3)])
+@pytest.mark.parametrize("index_dtype", [torch.int64, torch.int32])
+def test_the_number_of_rows_with_entries(N, K, index_dtype):
+    """Exactly, wherever in a row its only entry stands."""
+    torch.manual_seed(N + K)
+    V = 50
+    idx = torch.full((N, K), -1, dtype=index_dtype)
+    kind, at = torch.randint(0, 4, (N,)), torch.randint(0, K, (N,))
+    rows = torch.arange(N)
+    idx[rows, at] = torch.where(kind == 0, -7, torch.randint(0, V, (N,))).to(index_dtype)     # none
+    idx[kind == 1] = torch.randint(0, V, (int((kind == 1).sum()), K)).to(index_dtype)         # all
+    te = torch.randn(N, K)
+    te[rows[kind == 2], at[kind == 2]] = -math.inf                                            # one that the teacher excludes
+    want = ((idx >= 0) & (te != -math.inf)).any(1).sum()
+    z = torch.randn(N, V)
+    loss, stats, count = torch.ops.catch_b200.top_logits_distillation_stats(z.to(DEV), te.to(DEV), idx.to(DEV), 1.0, 1)
+    assert float(count[0]) == float(want)
+    each = torch.ops.catch_b200.top_logits_distillation(z.to(DEV), te.to(DEV), idx.to(DEV), 1.0, 0).cpu().double()
+    assert abs(float(loss) - float(each.sum()) / max(1, int(want))) <= (SLACK + N // 32) * cases.U * float(each.abs().sum()) / max(1, int(want))

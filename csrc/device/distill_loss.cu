@@ -436,12 +436,16 @@ bool valid(const B200Distill* p) {
          (p->index_dtype == B200_I64 || p->index_dtype == B200_I32) && (!p->loss || p->scratch);
 }
 
-// Threads for a row: 30 vectors for each, and at least half as many as there are kept entries.  Small blocks because a row's
-// reductions leave an SM idle unless others are at work (4096 x 30522 bf16 with gradient: 164 us in blocks of 512, 129 in blocks of 128);
-// not smaller, because more rows in work do not stay in L2 until their second pass (4096 x 131072: 534 us with 512, 603 with 256).
+// Threads for a row: at most 30 vectors for each, and at least half as many as there are kept entries.  Small blocks because a row's
+// reductions leave an SM idle unless others are at work; not smaller, because more rows in work do not stay in L2 until their second
+// pass.  Loss and gradient, us, with 128 / 256 / 512 threads (4096 rows, bf16): 24000 words 112 / 118 / 140, 31000 words (3875 vectors) 128 / 132 /
+// 151, 32000: 146 / 146 / 165, 40000: 191 / 175 / 192, 61000: 280 / 234 / 249, 65536 (8192 vectors): 329 / 276 / 278, 98304: 501 / 454 / 394; fp32, where 256
+// wins from 2800 vectors on: 10000 words 85 / 85 / 106, 15300 (3825): 122 / 116 / 132, 30522: 290 / 237 / 237, 35000: 331 / 286 / 265.  Fewer than 128
+// only where a row has no 64 vectors to give (65536 x 256 bf16, loss and loss with gradient, 32 / 64 / 128 threads: 202 / 177 / 183 and 230 / 237 /
+// 249; 16384 x 2000: 77 / 67 / 65 and 122 / 108 / 108).
 int row_threads(const B200Distill& p) {
   const long long vectors = p.V / (p.dtype == B200_F32 ? 4 : 8);
-  int t = 32;
+  int t = vectors > 64 ? 128 : 64;
   while (t < kMaxThreads && (vectors > 30LL * t || p.K > 2 * t)) t *= 2;
   return t;
 }

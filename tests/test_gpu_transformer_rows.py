@@ -123,7 +123,7 @@ def test_rotary_from_head_to_head(dtype, B, L, Hq, Hk, D, R, interleaved, packed
     (BF16, 2600, 20011, 40, None),      # two or three rows to a block of 128 threads
     (BF16, 1300, 33000, 64, "padded"),
     (F32, 2500, 9001, 16, None),
-    (BF16, 12000, 40, 7, None),         # to a block of one warp
+    (BF16, 12000, 40, 7, None),         # five to a block of two warps
     (F32, 11000, 33, 5, "padded"),
     (BF16, 700, 70001, 300, None),      # to a block of 512
 ])

@@ -640,7 +640,13 @@ struct BiasNode : public torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(2);
     if (!g[0].defined()) return out;
-    const Tensor s = scores.unpack(), t = table.unpack(), m = mask.unpack(), st = stats.unpack();
+    Tensor s = scores.unpack();
+    const Tensor t = table.unpack(), m = mask.unpack(), st = stats.unpack();
+    // A copy in the kernels' layout stands for the scores, also to whoever differentiates the gradient.
+    if (at::GradMode::is_enabled() && !s.requires_grad() && next_edge(0).is_valid()) {
+      s = s.detach();
+      torch::autograd::impl::set_gradient_edge(s, next_edge(0));
+    }
     refuse_captured_backward("relative_bias_softmax", s);
     static const auto op = find_op<decltype(relative_bias_softmax_backward)>("catch_b200::relative_bias_softmax_backward");
     std::tie(out[0], out[1]) =

@@ -195,3 +195,19 @@ def test_without_the_early_gradient_the_forward_holds_none(dtype, reduction):
             check(dz, *cases.distill_reference(z, t, idx, 2.0, reduction, factor)[1], "gradient")
             del dz
         del loss
+
+
+def test_second_derivatives_of_scores_that_are_laid_out_anew():
+    """The copy that the backward reads must not hide the scores from whoever differentiates once more."""
+    from catch_b200.fusion import relative_bias_softmax
+
+    wide = torch.randn(1, 2, 3, 9).to(DEV)
+    s = wide[..., 1:6].detach().requires_grad_()
+    y = relative_bias_softmax(s, torch.randn(8, 2).to(DEV), max_distance=8)
+    (d,) = torch.autograd.grad(y.square().sum(), s, create_graph=True)
+    with pytest.raises(RuntimeError, match="gradient of the gradient"):
+        torch.autograd.grad((d * s.detach()).sum() + s.sum(), s)
+    t = torch.randn(8, 2).to(DEV)
+    (d,) = torch.autograd.grad(relative_bias_softmax(s, t, max_distance=8), s, torch.ones(1, 2, 3, 5).to(DEV), create_graph=True)
+    with pytest.raises(RuntimeError, match="gradient of the gradient"):
+        torch.autograd.grad(d.sum() + s.sum(), s)

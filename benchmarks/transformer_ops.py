@@ -9,7 +9,6 @@ direction has to move: each tensor it reads and writes once; the rate is set aga
 import argparse
 import os
 import sys
-import time
 
 import torch
 
@@ -25,11 +24,13 @@ def timed(fn, sets, iters):
     for s in sets:
         fn(*s)
     torch.b200.synchronize()
-    t = time.perf_counter()
+    begin, end = (torch.b200.Event(enable_timing=True) for _ in range(2))
+    begin.record()
     for i in range(iters):
         fn(*sets[i % len(sets)])
+    end.record()
     torch.b200.synchronize()
-    return (time.perf_counter() - t) / iters * 1e6
+    return begin.elapsed_time(end) / iters * 1e3
 
 
 def report(name, us, bytes_):
@@ -54,7 +55,8 @@ def rotary(iters):
 
 def softmax(iters):
     for B, H, Lq, Lk, dt, mask in ((2, 12, 2048, 2048, bf16, None), (2, 12, 2048, 2048, bf16, "causal"), (128, 12, 128, 128, bf16, "padding"),
-                                   (16, 12, 512, 512, bf16, None), (12, 7, 389, 517, f32, "random")):
+                                   (16, 12, 512, 512, bf16, None), (12, 7, 389, 517, f32, "random"),
+                                   (1, 12, 1024, 8192, bf16, None), (1, 12, 1024, 16384, bf16, None), (1, 12, 1024, 8192, f32, None)):
         m = None
         if mask == "causal":
             m = torch.zeros(Lq, Lk).masked_fill(torch.arange(Lk) > torch.arange(Lq)[:, None], -float("inf")).to(dt).view(1, 1, Lq, Lk).to(DEV)
@@ -78,18 +80,23 @@ def softmax(iters):
 def distill(iters):
     from catch_b200.fusion import top_logits_distillation
 
-    for N, V, K, dt in ((4096, 30522, 64, bf16), (4096, 131072, 128, bf16), (777, 50021, 37, f32), (8192, 1000, 5, bf16)):
-        teacher, index = torch.randn(N, K).to(DEV), ((torch.randint(0, V, (N, 1)) + torch.arange(K) * (V // K)) % V).to(DEV)
+    for N, V, K, dt, absent in ((4096, 30522, 64, bf16, 0.0), (4096, 131072, 128, bf16, 0.0), (777, 50021, 37, f32, 0.0), (8192, 1000, 5, bf16, 0.0),
+                                (4096, 30522, 64, bf16, 0.85), (16384, 4000, 128, bf16, 0.85)):
+        index = (torch.randint(0, V, (N, 1)) + torch.arange(K) * (V // K)) % V
+        index[torch.rand(N) < absent] = -1
+        teacher, index = torch.randn(N, K).to(DEV), index.to(DEV)
         sets = [(torch.randn(N, V).to(dt).to(DEV),) for _ in range(2)]
         grad = [(z.clone().requires_grad_(),) for (z,) in sets]
         n = N * V * dt.itemsize
-        name = f"distill {N}x{V} kept {K} {str(dt)[6:]}"
-        loss = lambda z: top_logits_distillation(z, teacher, index, temperature=2.0)  # noqa: E731
+        name = f"distill {N}x{V} kept {K} {str(dt)[6:]}" + (f" {absent:.0%} of the rows empty" if absent else "")
+        loss = lambda z, early=True: top_logits_distillation(z, teacher, index, temperature=2.0, early_gradient=early)  # noqa: E731
         report(name + " loss", timed(loss, sets, iters), n)
         report(name + " loss and gradient", timed(loss, grad, iters), 2 * n)
         one = torch.ones(()).to(DEV)
         report(name + " with backward(), factor 1", timed(lambda z: torch.autograd.grad(loss(z), (z,), one), grad, iters), 2 * n)
-        report(name + " with backward(), factor 0.5", timed(lambda z: torch.autograd.grad(loss(z), (z,), 0.5 * one), grad, iters), 2 * n)
+        half = 0.5 * one
+        report(name + " with backward(), factor 0.5", timed(lambda z: torch.autograd.grad(loss(z), (z,), half), grad, iters), 2 * n)
+        report(name + " the same, early_gradient=False", timed(lambda z: torch.autograd.grad(loss(z, False), (z,), half), grad, iters), 2 * n)
 
 
 if __name__ == "__main__":

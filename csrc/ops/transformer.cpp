@@ -159,6 +159,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_backward_meta(const Te
           given(qw) && need_qw ? at::empty(qw->sizes(), qw->options()) : Tensor(), given(kw) && need_kw ? at::empty(kw->sizes(), kw->options()) : Tensor()};
 }
 
+// The kernels read a row's two statistics at once; a caller's may begin anywhere.
+Tensor by_pairs(const Tensor& stats) { return reinterpret_cast<uintptr_t>(stats.data_ptr()) % 8 == 0 ? stats : stats.clone(); }
 Tensor dense_last(const Tensor& t) { return t.stride(-1) == 1 || t.numel() == 0 ? t : t.contiguous(); }
 
 // The kernel's arguments that both directions share; `keep` holds what has to outlive the call.
@@ -603,11 +605,11 @@ std::tuple<Tensor, Tensor> relative_bias_softmax_backward(const Tensor& grad, co
   }
   OpScope scope("relative_bias_softmax_backward", a.scores);
   Tensor s = score_layout(a.scores), g = in_layout_of(grad, s), table = a.table.contiguous();
-  Tensor ds = fresh_strided(s), dt;
+  Tensor ds = fresh_strided(s), pairs = by_pairs(stats), dt;
   B200BiasSoftmax p = bias_params(a, s, table);
   p.grad = g.data_ptr();
   p.out = ds.data_ptr();
-  p.stats = stats.data_ptr<float>();
+  p.stats = pairs.data_ptr<float>();
   if (need_table) {
     dt = fresh(table.sizes(), table);
     p.dtable = dt.data_ptr();
@@ -833,13 +835,13 @@ Tensor distill_bwd(const DistillArgs& a, const Tensor& grad, const Tensor& stats
   if (!on_device(a.logits))
     return host_distill_grad(a, host_teacher(a), grad.to(at::kFloat).reshape({-1}).expand({N}) / count.to(at::kFloat));
   OpScope scope("top_logits_distillation_backward", a.logits);
-  Tensor z = row_layout(a.logits), teacher = a.teacher.contiguous(), index = a.index.contiguous(), g = grad.to(at::kFloat);
+  Tensor z = row_layout(a.logits), teacher = a.teacher.contiguous(), index = a.index.contiguous(), g = grad.to(at::kFloat), pairs = by_pairs(stats);
   B200Distill p = distill_params(a, z, teacher, index);
   // What backward() is given may lie elsewhere than what the forward saw (hooks on saved tensors, a recomputed forward): the kernel
   // takes the rows' place within 16 bytes from the logits.
   const bool keep = ready.defined() && in_phase(ready, z);
   Tensor out = keep ? ready : empty_in_phase(z, p.ld);
-  p.stats = stats.data_ptr<float>();
+  p.stats = pairs.data_ptr<float>();
   p.count = mean ? count.data_ptr<float>() : nullptr;
   p.dlogits = out.data_ptr();
   p.dlogits_ld = row_distance(out);

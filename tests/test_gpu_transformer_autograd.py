@@ -211,3 +211,21 @@ def test_second_derivatives_of_scores_that_are_laid_out_anew():
     (d,) = torch.autograd.grad(relative_bias_softmax(s, t, max_distance=8), s, torch.ones(1, 2, 3, 5).to(DEV), create_graph=True)
     with pytest.raises(RuntimeError, match="gradient of the gradient"):
         torch.autograd.grad(d.sum() + s.sum(), s)
+
+
+def test_statistics_may_begin_anywhere():
+    """A caller (or a hook on saved tensors) may keep them as a part of something else: on no boundary of a pair of numbers."""
+    ops = torch.ops.catch_b200
+
+    def elsewhere(t):
+        return torch.cat([torch.zeros(1, device=DEV), t.flatten()])[1:].view(t.shape)
+
+    s, t, g = torch.randn(2, 2, 5, 9).to(DEV), torch.randn(8, 2).to(DEV), torch.randn(2, 2, 5, 9).to(DEV)
+    p, st = ops.relative_bias_softmax(s, t, None, 1.0, True, 12, 0)
+    assert elsewhere(st).data_ptr() % 8 == 4 and elsewhere(st).is_contiguous()
+    a, b = (ops.relative_bias_softmax_backward(g, s, x, t, None, 1.0, True, 12, 0, True) for x in (st, elsewhere(st)))
+    assert torch.equal(a[0].cpu(), b[0].cpu()) and torch.equal(a[1].cpu(), b[1].cpu())
+    z, te, idx = torch.randn(5, 33).to(DEV), torch.randn(5, 3).to(DEV), torch.randint(0, 33, (5, 3)).to(DEV)
+    loss, st, count = ops.top_logits_distillation_stats(z, te, idx, 1.0, 1)
+    a, b = (ops.top_logits_distillation_backward(torch.ones(()).to(DEV), z, x, count, te, idx, 1.0, 1) for x in (st, elsewhere(st)))
+    assert torch.equal(a.cpu(), b.cpu())

@@ -812,7 +812,6 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
   int resident = resident_threads(pl.warps, bwd) / pl.threads;
   const int by_smem = (int)(220 * 1024 / (pl.smem + 1536));
   if (resident > by_smem) resident = by_smem > 0 ? by_smem : 1;
-  
   long long blocks = 148LL * resident / (p.H > 0 ? p.H : 1);
   const long long most = ((long long)a.rows + groups - 1) / groups;
   if (blocks > most) blocks = most;
@@ -827,7 +826,8 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
 template <typename K>
 int launch(K kernel, const Plan& pl, cudaStream_t s) {
   if (pl.smem > 48 * 1024 - 512) {  // beside the static part
-    const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem);
+    // the same limit in every call: another thread may be between this and its launch
+    const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
     if (e != cudaSuccess) return (int)e;
   }
   kernel<<<(unsigned)(pl.a.blocks_per_head * pl.a.H), pl.threads, pl.smem, s>>>(pl.a);

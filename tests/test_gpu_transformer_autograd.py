@@ -229,3 +229,34 @@ def test_statistics_may_begin_anywhere():
     loss, st, count = ops.top_logits_distillation_stats(z, te, idx, 1.0, 1)
     a, b = (ops.top_logits_distillation_backward(torch.ones(()).to(DEV), z, x, count, te, idx, 1.0, 1) for x in (st, elsewhere(st)))
     assert torch.equal(a.cpu(), b.cpu())
+
+
+def test_threads_with_tables_of_different_sizes():
+    """The same kernel at once with more and with less shared memory."""
+    import threading
+
+    ops = torch.ops.catch_b200
+    s, g, t = (torch.randn(1, 1, 1, 2048).bfloat16().to(DEV), torch.randn(1, 1, 1, 2048).bfloat16().to(DEV), torch.randn(32, 1).to(DEV))
+    forward = lambda d: ops.relative_bias_softmax(s, t, None, 1.0, True, d, 9000)  # noqa: E731
+    backward = lambda d, st: ops.relative_bias_softmax_backward(g, s, st, t, None, 1.0, True, d, 9000, True)  # noqa: E731
+    want = {d: (forward(d)[0].cpu(), *(x.cpu() for x in backward(d, forward(d)[1]))) for d in (8192, 4096)}
+    errors = []
+
+    def work(d):
+        try:
+            with torch.b200.stream(torch.b200.queue_from_pool()):
+                for _ in range(30000):
+                    p, st = forward(d)
+                for _ in range(5000):
+                    grads = backward(d, st)
+                assert all(torch.equal(a.cpu(), b) for a, b in zip((p, *grads), want[d]))
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    torch.b200.synchronize()
+    threads = [threading.Thread(target=work, args=(d,)) for d in (8192, 4096, 8192, 4096)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not errors, errors

@@ -774,7 +774,7 @@ B200Distill distill_params(const DistillArgs& a, const Tensor& z, const Tensor& 
   return p;
 }
 
-// (loss, statistics [rows, 2], number of rows that count [1], gradient of the logits for a factor of 1 or undefined)
+// (loss, statistics [rows, 2], number of rows that count with the kernels' scratch behind it, gradient of the logits for a factor of 1 or undefined)
 std::tuple<Tensor, Tensor, Tensor, Tensor> distill_fwd(const DistillArgs& a, bool need_grad) {
   check_distill(a);
   const bool mean = a.reduction == at::Reduction::Mean, each = a.reduction == at::Reduction::None;
@@ -787,9 +787,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> distill_fwd(const DistillArgs& a, boo
     if (h.at.size(1) > 0)
       rows = rows - (h.share * (z.gather(1, h.at) - lse.unsqueeze(1))).masked_fill(h.share.eq(0), 0.0).sum(1);
     rows = (rows * (a.temperature * a.temperature)).masked_fill(h.rows.logical_not(), 0.0);
-    Tensor count = mean ? h.rows.sum().to(at::kFloat).clamp_min(1.0).reshape({1}) : at::ones({1}, fopt);
-    Tensor loss = each ? rows : rows.sum() / count.squeeze(0);
-    Tensor grad = need_grad && !each ? host_distill_grad(a, h, count.reciprocal().expand({N})) : Tensor();
+    Tensor count = mean ? h.rows.sum().to(at::kFloat).reshape({1}) : at::ones({1}, fopt);
+    Tensor loss = each ? rows : rows.sum() / count.clamp_min(1.0).squeeze(0);
+    Tensor grad = need_grad && !each ? host_distill_grad(a, h, count.clamp_min(1.0).reciprocal().expand({N})) : Tensor();
     return {loss, at::stack({lse, lse}, 1), count, grad};
   }
   OpScope scope("top_logits_distillation", a.logits);
@@ -833,7 +833,7 @@ Tensor distill_bwd(const DistillArgs& a, const Tensor& grad, const Tensor& stats
   const bool mean = a.reduction == at::Reduction::Mean, each = a.reduction == at::Reduction::None;
   const int64_t N = a.logits.size(0);
   if (!on_device(a.logits))
-    return host_distill_grad(a, host_teacher(a), grad.to(at::kFloat).reshape({-1}).expand({N}) / count.to(at::kFloat));
+    return host_distill_grad(a, host_teacher(a), grad.to(at::kFloat).reshape({-1}).expand({N}) / count.to(at::kFloat).clamp_min(1.0));
   OpScope scope("top_logits_distillation_backward", a.logits);
   Tensor z = row_layout(a.logits), teacher = a.teacher.contiguous(), index = a.index.contiguous(), g = grad.to(at::kFloat), pairs = by_pairs(stats);
   B200Distill p = distill_params(a, z, teacher, index);
@@ -861,6 +861,8 @@ Tensor top_logits_distillation(const Tensor& logits, const Tensor& teacher, cons
 std::tuple<Tensor, Tensor, Tensor> top_logits_distillation_stats(const Tensor& logits, const Tensor& teacher, const Tensor& index,
                                                                  double temperature, int64_t reduction) {
   auto [loss, stats, count, ready] = distill_fwd({logits, teacher, index, temperature, reduction}, false);
+  count = count.narrow(0, 0, 1);  // (behind it: the kernels' scratch)
+  if (reduction != at::Reduction::Mean || logits.size(0) == 0) count.fill_(reduction != at::Reduction::Mean);
   return {loss, stats, count};
 }
 Tensor top_logits_distillation_backward(const Tensor& grad, const Tensor& logits, const Tensor& stats, const Tensor& count, const Tensor& teacher,
@@ -876,7 +878,7 @@ Tensor top_logits_distillation_meta(const Tensor& logits, const Tensor& teacher,
 std::tuple<Tensor, Tensor, Tensor> top_logits_distillation_stats_meta(const Tensor& logits, const Tensor& teacher, const Tensor& index,
                                                                       double temperature, int64_t reduction) {
   Tensor loss = top_logits_distillation_meta(logits, teacher, index, temperature, reduction, false);
-  return {loss, at::empty({logits.size(0), 2}, loss.options()), at::empty({on_device(logits) ? 1 + B200_DISTILL_SCRATCH : 1}, loss.options())};
+  return {loss, at::empty({logits.size(0), 2}, loss.options()), at::empty({1}, loss.options())};
 }
 Tensor top_logits_distillation_backward_meta(const Tensor& grad, const Tensor& logits, const Tensor& stats, const Tensor& count, const Tensor& teacher,
                                              const Tensor& index, double temperature, int64_t reduction) {

@@ -260,3 +260,9 @@ def test_threads_with_tables_of_different_sizes():
     for thread in threads:
         thread.join()
     assert not errors, errors
+
+
+def test_numbers_of_rows():
+    from test_transformer_ops_more import numbers_of_rows
+
+    numbers_of_rows(DEV)

@@ -309,3 +309,27 @@ def test_an_encoder_takes_configurations_from_before_there_were_position_types()
     b.load_state_dict(a.state_dict())
     ids = torch.randint(0, 50, (2, 7))
     assert torch.equal(a(ids), b(ids))
+
+
+def numbers_of_rows(dev):
+    """The third result is the number of rows with entries for a mean, 1 otherwise, and nothing else."""
+    ops = torch.ops.catch_b200
+    for n, kept, want in ((4, [[0, -1], [-1, -1], [2, 3], [-1, 1]], 3), (2, [[-1, -1], [-5, -1]], 0), (0, [], 0)):
+        z, te = torch.randn(n, 5).to(dev), torch.randn(n, 2).to(dev)
+        idx = torch.tensor(kept, dtype=torch.long).view(n, 2).to(dev)
+        for reduction in (0, 1, 2):
+            loss, stats, count = ops.top_logits_distillation_stats(z, te, idx, 2.0, reduction)
+            assert count.shape == (1,) and float(count) == (want if reduction == 1 else 1), (n, reduction, count)
+            assert bool(torch.isfinite(loss.cpu()).all())
+            leaf = z.clone().requires_grad_()
+            (dz,) = torch.autograd.grad(ops.top_logits_distillation(leaf, te, idx, 2.0, reduction).sum(), leaf)
+            g = torch.ones(loss.shape).to(dev)
+            assert torch.equal(ops.top_logits_distillation_backward(g, z, stats, count, te, idx, 2.0, reduction).cpu(), dz.cpu())
+            # the same numbers on the host
+            host = ops.top_logits_distillation_stats(z.cpu(), te.cpu(), idx.cpu(), 2.0, reduction)
+            assert torch.equal(host[2], count.cpu())
+
+
+@pytest.mark.parametrize("dev", ["cpu", "blackwell"])
+def test_numbers_of_rows(dev):
+    numbers_of_rows(dev)

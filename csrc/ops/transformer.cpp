@@ -499,8 +499,7 @@ std::tuple<Tensor, Tensor> host_logits(const BiasArgs& a) {
   return {x, bucket};
 }
 Tensor host_probs(const Tensor& x, const Tensor& stats) {
-  Tensor p = at::exp(x - stats.select(-1, 0).unsqueeze(-1)) * stats.select(-1, 1).unsqueeze(-1);
-  return p.masked_fill(x.eq(-kInf), 0.0);
+  return at::exp(x - stats.select(-1, 0).unsqueeze(-1)) * stats.select(-1, 1).unsqueeze(-1);  // x = -inf: 0, in a NaN row NaN
 }
 
 bool sixteen(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
@@ -549,7 +548,8 @@ std::tuple<Tensor, Tensor> relative_bias_softmax(const Tensor& scores, const Ten
     if (a.scores.numel() == 0) return {at::empty_like(a.scores), at::empty(ss, a.scores.options().dtype(at::kFloat))};
     auto [x, bucket] = host_logits(a);
     Tensor m = std::get<0>(x.max(-1));
-    Tensor e = at::exp(x - m.unsqueeze(-1)).masked_fill(x.eq(-kInf), 0.0);
+    m = m.masked_fill(m.eq(-kInf), 0.0);  // a row with nothing left
+    Tensor e = at::exp(x - m.unsqueeze(-1));
     Tensor sum = e.sum(-1), inv = at::where(sum.eq(0), at::zeros_like(sum), sum.reciprocal());
     Tensor stats = at::stack({m, inv}, -1);
     return {host_probs(x, stats).to(a.scores.scalar_type()), stats};
@@ -785,7 +785,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> distill_fwd(const DistillArgs& a, boo
     Tensor z = a.logits.to(at::kFloat) / a.temperature, lse = at::logsumexp(z, 1);
     Tensor rows = h.plogp;
     if (h.at.size(1) > 0)
-      rows = rows - (h.share * (z.gather(1, h.at) - lse.unsqueeze(1))).masked_fill(h.share.eq(0), 0.0).sum(1);
+      rows = rows - (h.share * at::log_softmax(z, 1).gather(1, h.at)).masked_fill(h.share.eq(0), 0.0).sum(1);
     rows = (rows * (a.temperature * a.temperature)).masked_fill(h.rows.logical_not(), 0.0);
     Tensor count = mean ? h.rows.sum().to(at::kFloat).reshape({1}) : at::ones({1}, fopt);
     Tensor loss = each ? rows : rows.sum() / count.clamp_min(1.0).squeeze(0);

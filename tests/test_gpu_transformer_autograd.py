@@ -266,3 +266,9 @@ def test_numbers_of_rows():
     from test_transformer_ops_more import numbers_of_rows
 
     numbers_of_rows(DEV)
+
+
+def test_infinities_and_nan():
+    from test_transformer_ops_more import infinities_and_nan
+
+    infinities_and_nan(DEV)

@@ -333,3 +333,30 @@ def numbers_of_rows(dev):
 @pytest.mark.parametrize("dev", ["cpu", "blackwell"])
 def test_numbers_of_rows(dev):
     numbers_of_rows(dev)
+
+
+def infinities_and_nan(dev):
+    """Kept scores and logits that are infinite or no number give what torch's softmax gives for the row: NaN throughout."""
+    from catch_b200.fusion import relative_bias_softmax, top_logits_distillation
+
+    for bad in (math.inf, math.nan):
+        for Lk in (5, 64, 1100):
+            s = torch.randn(1, 1, 3, Lk)
+            s[0, 0, 1, 2] = bad
+            m = torch.ones(1, 1, 3, Lk, dtype=torch.bool)
+            m[..., 0] = False
+            p = relative_bias_softmax(s.to(dev), torch.zeros(4, 1).to(dev), m.to(dev), max_distance=8).cpu()
+            want = torch.softmax(s.masked_fill(~m, -math.inf), -1)
+            assert torch.equal(p.isnan(), want.isnan()) and bool(want[0, 0, 1].isnan().all())
+            assert torch.allclose(p, want, rtol=1e-5, atol=1e-7, equal_nan=True)
+        z = torch.randn(3, 70)
+        z[1, 7] = bad
+        idx = torch.tensor([[0, 7], [3, 4], [5, 6]])
+        loss = top_logits_distillation(z.to(dev), torch.zeros(3, 2).to(dev), idx.to(dev), reduction="none").cpu()
+        want = math.log(0.5) - torch.log_softmax(z, 1).gather(1, idx).mean(1)
+        assert torch.allclose(loss, want, rtol=1e-5, atol=1e-6, equal_nan=True) and bool(loss[1].isnan())
+
+
+@pytest.mark.parametrize("dev", ["cpu", "blackwell"])
+def test_infinities_and_nan(dev):
+    infinities_and_nan(dev)

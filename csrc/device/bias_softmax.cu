@@ -18,7 +18,9 @@
 // the scores alone and 118 us with the table = 5.1 TB/s, 0.78; with a causal mask of 16 bits 117 and 180 us.  128 x 12 x 128 x 128 bf16 with an
 // fp32 padding mask: 38 and 70 us (2.6 and 2.1 TB/s), where every distance is a near one.  Issue slots are what it runs out of (68 % and 63 %
 // busy at 2048 keys; 18 and 23 instructions an element), and unaligned fp32 rows of 517 keys with a random bool mask run at 1.2 to 1.5 TB/s
-// for the same reason.
+// for the same reason.  Rows beyond the registers read the scores twice in each direction: 12 x 1024 x 16384 bf16 270 us forward, 712 backward
+// for the scores, 737 with the table (0.45 and 0.25 of the copy), 12 x 1024 x 8192 fp32 212, 430 and 445 us; 12 x 1024 x 8192 bf16, the
+// longest in registers, 95, 119 and 148 us.
 #include "kernels_api.h"
 #include "row_vec.cuh"
 
@@ -786,7 +788,7 @@ Plan make_plan(const B200BiasSoftmax& p, bool bwd) {
   int groups = 1;
   // 16 elements in a lane: fewer and the reductions and addresses of a row are too much for them, more and there are too few rows at once
   // (2048 keys in one / two / four / eight warps, before rows were copied ahead: forward 184 / 112 / 107 / 138 us, backward 530 / 271 / 172 /
-  // 184 us).  Rows beyond eight warps of these take 32 elements a lane, and from 8192 keys of 16 bits (4096 of 32) on two passes.
+  // 184 us).  Rows beyond eight warps of these take 32 elements a lane, and beyond 8192 keys of 16 bits (4096 of 32) two passes.
   const int wide = 16 / vec;  // vectors for 16 elements
   if (nvec <= 32 * wide) {
     int G = 1;

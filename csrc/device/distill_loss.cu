@@ -10,10 +10,12 @@
 // factor that backward() begins with, 1 (over the number of rows for a mean).  When another factor arrives, the backward writes dz anew
 // from z and the two saved numbers of each row, so that every gradient is rounded once whatever the factor.
 //
-// Measured on a B200, bf16, loss and gradient: 4096 x 30522, 64 kept: 127 us = 3.9 TB/s, 0.60 of the measured copy bandwidth; 4096 x 131072,
-// 128 kept: 547 us = 3.9 TB/s, 0.60; the loss alone 64 us (3.9 TB/s) and 214 us (5.0 TB/s).  With a factor other than 1 the early gradient was
-// written for nothing: 235 us with the backward at 4096 x 30522, where the loss alone (64) and the backward (102) are 166.  What bounds the
-// pass: issue slots (72 % busy) at 30522 words; at 131072 also L2, where half of the second reading misses.
+// Measured on a B200, bf16, loss and gradient: 4096 x 30522, 64 kept: 128 us = 3.9 TB/s, 0.60 of the measured copy bandwidth; 4096 x 131072,
+// 128 kept: 530 us = 4.1 TB/s, 0.62; the loss alone 64 us (3.9 TB/s) and 213 us (5.0 TB/s).  With a factor other than 1 the early gradient was
+// written for nothing: 231 us with the backward at 4096 x 30522; a caller who knows leaves it out (163 us: the loss and a pass of its own).
+// What bounds the pass: issue slots (72 % busy) at 30522 words; at 131072 also L2, where half of the second reading misses.  Many short
+// rows are bound by their reductions and by the last block's sum over them: 8192 x 1000, 5 kept, 31 us for the loss, 40 with its gradient, 0.08
+// and 0.13 of the copy.
 #include "kernels_api.h"
 #include "row_vec.cuh"
 

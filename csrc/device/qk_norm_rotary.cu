@@ -15,10 +15,11 @@
 // of one token and keeps the token's cos / sin and the weight in registers, while its next heads are copied to shared memory.
 //
 // Measured on a B200 (bf16, queries of 32 and keys of 8 heads of 128 at 8 x 2048 tokens, slices of a packed projection): forward 68 us =
-// 5.0 TB/s, 0.76 of the measured copy bandwidth (82 us with loads that waited for the head before); backward with the weights' gradients
-// 123 us = 4.1 TB/s, 0.62 (178 us).  What bounds it there is issue slots (71 % and 61 % busy), not memory.  fp32, 16 + 16 heads of 64: 50 and
-// 74 us = 5.3 and 5.5 TB/s.  Head dimensions that leave lanes of a group idle or narrow the vectors run at 1.3 to 2.5 TB/s (80: five of
-// eight lanes; 100: vectors of two).
+// 4.9 TB/s, 0.75 of the measured copy bandwidth (82 us with loads that waited for the head before), where issue slots run out (70 %
+// busy); backward with the weights' gradients 126 us = 4.0 TB/s, 0.61 (178 us).  The backward is short of warps: 121 registers leave two
+// blocks of 256 threads on an SM, 24 % of its warps, which keep 60 % of the issue slots busy.  fp32, 16 + 16 heads of 64: 50 and 74 us =
+// 5.4 and 5.5 TB/s.  Head dimensions that leave lanes of a group idle or narrow the vectors run at 1.3 to 2.5 TB/s (80: five of eight
+// lanes; 100: vectors of two).
 #include "kernels_api.h"
 #include "row_vec.cuh"
 

@@ -272,3 +272,39 @@ def test_infinities_and_nan():
     from test_transformer_ops_more import infinities_and_nan
 
     infinities_and_nan(DEV)
+
+
+@pytest.mark.parametrize("how", ["checkpoint", "reentrant checkpoint", "on the host"])
+def test_recomputed_and_offloaded_tensors(how):
+    """The three operators in a row, their saved tensors recomputed or kept on the host meanwhile."""
+    from catch_b200.fusion import qk_norm_rotary, relative_bias_softmax, top_logits_distillation
+    from torch.utils.checkpoint import checkpoint
+
+    torch.manual_seed(4)
+    B, L, H, D, V = 2, 11, 3, 16, 77
+    qkv, w, table = torch.randn(B, L, 3 * H, D), torch.ones(D), torch.randn(8, H)
+    head = torch.randn(H * D, V + 6)
+    cos, sin = (t.to(DEV) for t in cases.tables(L, D))
+    t, idx = (x.to(DEV) for x in cases.teacher_of(B * L, V, 5, 1))
+
+    def body(qkv, w, table, head):
+        q, k = qk_norm_rotary(qkv[:, :, :H], qkv[:, :, H:2 * H], w, w, cos, sin)
+        p = relative_bias_softmax(torch.matmul(q.permute(0, 2, 1, 3), k.permute(0, 2, 3, 1)), table, scale=0.25, max_distance=12)
+        y = torch.matmul(p, qkv[:, :, 2 * H:].permute(0, 2, 1, 3)).permute(0, 2, 1, 3).reshape(B * L, H * D)
+        return top_logits_distillation(torch.matmul(y, head)[:, 3:3 + V], t, idx, temperature=2.0)
+
+    def leaves():
+        return [x.to(DEV).requires_grad_() for x in (qkv, w, table, head)]
+
+    plain, other = leaves(), leaves()
+    (body(*plain)).backward()
+    for factor in (1.0, 0.5):
+        for x in other:
+            x.grad = None
+        if how == "on the host":
+            with torch.autograd.graph.save_on_cpu():
+                (factor * body(*other)).backward()
+        else:
+            (factor * checkpoint(body, *other, use_reentrant=how.startswith("reentrant"))).backward()
+        for a, b in zip(plain, other):
+            assert torch.allclose(factor * a.grad.cpu(), b.grad.cpu(), rtol=2.0 ** -18, atol=2.0 ** -18 * float(a.grad.cpu().abs().max()))
